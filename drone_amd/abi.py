@@ -6,6 +6,7 @@ has no binding source (``/root/reference/.gitmodules:1-3`` names an empty
 submodule).
 """
 import ctypes as C
+import struct
 
 OBS_DIM = 20
 OBS_DIM_MAX = 24
@@ -76,6 +77,57 @@ class DroneStateRow(C.Structure):
     ]
 
 
+# The policy operators: element types, activations, and the argument blocks of the calls.
+F32, BF16, F16 = 0, 1, 2
+ACTIVATIONS = {"none": 0, "relu": 1, "tanh": 2, "silu": 3, "gelu": 4}
+
+_V, _I64 = C.c_void_p, C.c_int64
+
+
+class DroneLinear(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("device", C.c_int32), ("dtype", C.c_int32), ("activation", C.c_int32),
+        ("rows", _I64), ("in_features", _I64), ("out_features", _I64),
+        ("x", _V), ("weight", _V), ("bias", _V), ("residual", _V), ("dy", _V),
+        ("y", _V), ("slope", _V), ("dx", _V), ("dweight", _V), ("dbias", _V),
+        ("x_ld", _I64), ("weight_ld", _I64), ("residual_ld", _I64), ("dy_ld", _I64), ("y_ld", _I64), ("dx_ld", _I64),
+        ("workspace", _V), ("workspace_bytes", C.c_uint64),
+    ]
+
+
+class DroneNorm(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("device", C.c_int32), ("dtype", C.c_int32), ("gate_kind", C.c_int32),
+        ("rows", _I64), ("width", _I64),
+        ("x", _V), ("block", _V), ("gate", _V), ("post_weight", _V), ("pre_weight", _V), ("dr", _V), ("dh", _V),
+        ("r", _V), ("h", _V), ("dx", _V), ("dblock", _V), ("dgate", _V), ("dpost_weight", _V), ("dpre_weight", _V),
+        ("x_ld", _I64), ("block_ld", _I64), ("gate_ld", _I64),
+        ("scale", _F), ("eps", _F),
+        ("workspace", _V), ("workspace_bytes", C.c_uint64),
+    ]
+
+
+class DroneAdamWTensor(C.Structure):
+    _fields_ = [("param", _V), ("grad", _V), ("exp_avg", _V), ("exp_avg_sq", _V), ("master", _V), ("elements", _I64)]
+
+
+class DroneAdamW(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("device", C.c_int32), ("dtype", C.c_int32), ("count", C.c_int32),
+        ("tensors", C.POINTER(DroneAdamWTensor)), ("step", _V), ("grad_norm", _V),
+        ("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double), ("max_grad_norm", C.c_double),
+        ("workspace", _V), ("workspace_bytes", C.c_uint64),
+    ]
+
+
+# The same blocks as struct formats: one pack() builds a call's bytes (the calls take any pointer), a tenth of the time of
+# filling a ctypes structure field by field.
+LINEAR_CALL = struct.Struct("@Iiii3q10P6qPQ")
+NORM_CALL = struct.Struct("@Iiii2q14P3q2fPQ")
+ADAMW_TENSOR = struct.Struct("@5Pq")
+ADAMW_CALL = struct.Struct("@Iiii3P6dPQ")
+
+
 # numpy structured dtype with the same layout as DroneStateRow (33 words).
 def state_row_dtype():
     import numpy as np
@@ -138,6 +190,14 @@ SYMBOLS = {
     "drone_device_malloc": (_P, [C.c_int, C.c_size_t]),
     "drone_device_free": (None, [C.c_int, _P]),
     "drone_vec_copy_to_host": (C.c_int, [_P, _P, _P, C.c_size_t]),
+    "drone_linear_forward": (C.c_int, [_P, _P]),
+    "drone_linear_backward": (C.c_int, [_P, _P]),
+    "drone_linear_workspace": (C.c_uint64, [_P]),
+    "drone_norm_forward": (C.c_int, [_P, _P]),
+    "drone_norm_backward": (C.c_int, [_P, _P]),
+    "drone_norm_workspace": (C.c_uint64, [_P]),
+    "drone_adamw_step": (C.c_int, [_P, _P]),
+    "drone_adamw_workspace": (C.c_uint64, [_P]),
     "drone_vec_timer_start": (C.c_int, [_P]),
     "drone_vec_timer_stop": (C.c_int, [_P, C.POINTER(C.c_float)]),
     "drone_last_error": (C.c_char_p, []),

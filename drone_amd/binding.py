@@ -46,6 +46,12 @@ def last_error():
     return _fns["drone_last_error"]().decode()
 
 
+def functions():
+    """The library's function table (``abi.SYMBOLS``), loaded on first use."""
+    load()
+    return _fns
+
+
 def default_config(task=abi.TASK_HOVER, **overrides):
     load()
     cfg = abi.DroneConfig()

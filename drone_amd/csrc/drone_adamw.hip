@@ -1,0 +1,137 @@
+// drone_adamw.hip — one AdamW step over many tensors with the clip by the global norm of their gradients:
+//   norm = sqrt(sum g^2);  c = min(1, max_norm / (norm + 1e-6));  g' = c g
+//   m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2
+//   p = p (1 - lr wd) - lr (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps)
+// Two launches whatever the number of tensors (up to kAdamwTensors): the norm's partial sums (and the step counter, in HBM
+// so that a captured step replays with an advancing t), then the update. Everything in 32 bits; a 16-bit weight is its
+// 32-bit master rounded once, and the master is what the next step starts from.
+#include <hip/hip_runtime.h>
+
+#include "drone_policy.hpp"
+
+#include "../../include/drone_vec.h"
+
+namespace drone {
+namespace {
+
+constexpr int kThreads = 256;
+
+// Which of the launch's tensors holds a chunk: every lane of the wave looks at one first_chunk of the table.
+__device__ __forceinline__ int tensor_of(const AdamwArgs& a, int chunk) {
+    const int lane = threadIdx.x & 63;
+    const unsigned long long mine = __ballot(lane < a.count && a.t[lane < a.count ? lane : 0].first_chunk <= chunk);
+    return __builtin_amdgcn_readfirstlane(__popcll(mine) - 1);
+}
+
+template <class T>
+__device__ __forceinline__ void load8(const T* p, long long i, long long n, bool vec, float* f) {
+    if (vec && i + 8 <= n) {
+        struct Eight { T e[8]; };
+        const Eight v = *(const Eight*)__builtin_assume_aligned(p + i, 16);
+#pragma unroll
+        for (int k = 0; k < 8; k++) f[k] = (float)v.e[k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; k++) f[k] = i + k < n ? (float)p[i + k] : 0.f;
+    }
+}
+
+template <class T>
+__device__ __forceinline__ void store8(T* p, long long i, long long n, bool vec, const float* f) {
+    if (vec && i + 8 <= n) {
+        struct Eight { T e[8]; } v;
+#pragma unroll
+        for (int k = 0; k < 8; k++) v.e[k] = (T)f[k];
+        *(Eight*)__builtin_assume_aligned(p + i, 16) = v;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; k++) if (i + k < n) p[i + k] = (T)f[k];
+    }
+}
+
+__device__ __forceinline__ float block_sum(float v, float* join) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    if ((threadIdx.x & 63) == 0) join[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return join[0] + join[1] + join[2] + join[3];
+}
+
+// partial[0..1]: the two bias corrections of this step; partial[2 + k]: the sums of squares
+template <class T>
+__global__ __launch_bounds__(kThreads) void adamw_norm_kernel(AdamwArgs a) {
+    __shared__ float join[4];
+    if (a.advance && blockIdx.x == 0 && threadIdx.x == 0) {
+        const int t = *a.step + 1;
+        *a.step = t;
+        a.partial[0] = (float)(1.0 - pow(a.b1d, (double)t));
+        a.partial[1] = (float)(1.0 - pow(a.b2d, (double)t));
+        if (a.norm && !a.chunks) *a.norm = 0.f;  // no gradients at all
+    }
+    if (!a.parts) return;
+    float sum = 0.f;
+    for (int chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
+        const AdamwTensor& t = a.t[tensor_of(a, chunk)];
+        float g[8];
+        load8((const T*)t.g, (long long)(chunk - t.first_chunk) * kAdamwChunk + threadIdx.x * 8, t.n, t.vec, g);
+#pragma unroll
+        for (int k = 0; k < 8; k++) sum += g[k] * g[k];
+    }
+    sum = block_sum(sum, join);
+    if (threadIdx.x == 0) a.partial[2 + a.part0 + blockIdx.x] = sum;
+}
+
+template <class T>
+__global__ __launch_bounds__(kThreads) void adamw_update_kernel(AdamwArgs a) {
+    __shared__ float join[4];
+    const int chunk = blockIdx.x;
+    const AdamwTensor& t = a.t[tensor_of(a, chunk)];
+    const long long i = (long long)(chunk - t.first_chunk) * kAdamwChunk + threadIdx.x * 8;
+    float g[8], m[8], v[8], p[8];
+    load8((const T*)t.g, i, t.n, t.vec, g);
+    load8(t.m, i, t.n, t.vec, m);
+    load8(t.v, i, t.n, t.vec, v);
+    if (t.master) load8(t.master, i, t.n, t.vec, p); else load8((const T*)t.p, i, t.n, t.vec, p);
+    float clip = 1.f;
+    if (a.parts) {  // every workgroup joins the partial sums in the same order
+        float sum = 0.f;
+        for (int k = threadIdx.x; k < a.parts; k += kThreads) sum += a.partial[2 + k];
+        const float norm = sqrtf(block_sum(sum, join));
+        if (a.max_norm > 0.f) {
+            clip = fminf(a.max_norm / (norm + 1e-6f), 1.f);
+            if (norm != norm) clip = norm;  // fminf drops a NaN; a step on NaN gradients has to show
+        }
+        if (a.norm && chunk == 0 && threadIdx.x == 0 && a.advance) *a.norm = norm;
+    }
+    const float c1 = a.partial[0], c2 = a.partial[1];
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        const float d = g[k] * clip;
+        m[k] = a.b1 * m[k] + a.rest1 * d;
+        v[k] = a.b2 * v[k] + a.rest2 * d * d;
+        p[k] = p[k] * a.decay - a.lr * (m[k] / c1) / (sqrtf(v[k] / c2) + a.eps);
+    }
+    store8(t.m, i, t.n, t.vec, m);
+    store8(t.v, i, t.n, t.vec, v);
+    if (t.master) store8(t.master, i, t.n, t.vec, p);
+    store8((T*)t.p, i, t.n, t.vec, p);
+}
+
+}  // namespace
+
+int adamw_norm_launch(int dtype, const AdamwArgs& a, int blocks, hipStream_t s) {
+    if (dtype == DRONE_F32) adamw_norm_kernel<float><<<blocks, kThreads, 0, s>>>(a);
+    else if (dtype == DRONE_BF16) adamw_norm_kernel<__bf16><<<blocks, kThreads, 0, s>>>(a);
+    else adamw_norm_kernel<_Float16><<<blocks, kThreads, 0, s>>>(a);
+    return (int)hipGetLastError();
+}
+
+int adamw_update_launch(int dtype, const AdamwArgs& a, hipStream_t s) {
+    if (!a.chunks) return 0;
+    if (dtype == DRONE_F32) adamw_update_kernel<float><<<a.chunks, kThreads, 0, s>>>(a);
+    else if (dtype == DRONE_BF16) adamw_update_kernel<__bf16><<<a.chunks, kThreads, 0, s>>>(a);
+    else adamw_update_kernel<_Float16><<<a.chunks, kThreads, 0, s>>>(a);
+    return (int)hipGetLastError();
+}
+
+}  // namespace drone

@@ -124,6 +124,48 @@ class Drone:
                 infos.append(log)
         return bufs.observations, bufs.rewards, bufs.terminals, bufs.truncations, infos
 
+    def collect(self, policy, k_steps):
+        """K steps with ``policy`` acting, everything on the GPU: the path a learner collects its batch with. ``policy`` is
+        a ``drone_amd.policy.Policy`` or any callable ``policy(observations, out=actions)`` that writes ``out``; it reads
+        the env's current observations and its actions go straight into the block the env steps from. Returns K-major
+        ``(observations [K][N][O] the policy saw, actions [K][N][4], rewards, terminals, truncations [K][N], infos)``; the
+        blocks are reused from call to call for the same K. Afterwards the env and its per-step buffers are where K calls of
+        ``step`` leave them. Device buffers only; capturable after ``vec.enable_graph_capture`` (one call outside first)."""
+        import torch
+
+        vec, K = self.vec, int(k_steps)
+        if vec.torch_device is None:
+            raise ValueError("collect needs an env with device buffers (device=...)")
+        if K < 1:
+            raise ValueError("k_steps must be at least 1")
+        bufs = getattr(self, "_collected", None)
+        if bufs is None or bufs.k_steps != K:
+            bufs = self._collected = vec.alloc_step_many(K)
+        own = vec.actions, (vec.observations, vec.rewards, vec.terminals, vec.truncations)
+        vec.use_torch_stream()
+        try:
+            with torch.no_grad():
+                bufs.observations[0].copy_(own[1][0])
+                for k in range(K):
+                    policy(bufs.observations[k], out=bufs.actions[k])
+                    vec.bind_actions(bufs.actions[k])
+                    vec.bind_outputs(bufs.observations[k + 1] if k + 1 < K else own[1][0], bufs.rewards[k], bufs.terminals[k], bufs.truncations[k])
+                    vec.step()
+                own[0].copy_(bufs.actions[K - 1])
+                for mine, block in zip(own[1][1:], (bufs.rewards, bufs.terminals, bufs.truncations)):
+                    mine.copy_(block[K - 1])
+        finally:
+            vec.bind_actions(own[0])
+            vec.bind_outputs(*own[1])
+        before = self.tick
+        self.tick += K
+        infos = []
+        if self.log_interval and before // self.log_interval != self.tick // self.log_interval:
+            log = vec.log()
+            if log["n"] > 0:
+                infos.append(log)
+        return bufs.observations, bufs.actions, bufs.rewards, bufs.terminals, bufs.truncations, infos
+
     def save(self, path):
         """Checkpoint the env (state, step counter, seed, config, buffer contents): ``DroneVec.save_checkpoint``."""
         self.vec.save_checkpoint(path)

@@ -8,7 +8,9 @@ then with "policy forward + env step" captured ONCE into a hipGraph
 keeps the step counter in HBM so the replays advance it. Last: the same graph
 with a frame skip of 4 — one policy forward, then four env steps under that
 action in ONE launch (drone_vec_step_repeat), the policy reading the last of the
-four observation blocks.
+four observation blocks. Then the same loop with the library's own layers
+(drone_amd.policy: one launch a layer), and a learner on top of it: Drone.collect,
+the gradient, one AdamW step.
 
     python examples/torch_policy_loop.py [--envs 65536] [--steps 500] [--task hover]
 """
@@ -111,6 +113,55 @@ def main():
     assert vec.gstep == g0 + calls * K
     print(f"frame skip {K} (one policy forward + drone_vec_step_repeat per replay): {a.envs * calls * K / el:.3e} env-steps/s "
           f"({el * 1e6 / (calls * K):.1f} us per env step, {el * 1e6 / calls:.1f} us per policy step)")
+
+    # the same network on the library's own layers (drone_amd.policy), captured the same way: four launches a step
+    from drone_amd.policy import AdamW, Policy
+
+    policy = Policy(vec.observations.shape[1], a.hidden, device=dev)
+    with torch.no_grad():
+        with torch.cuda.stream(side):
+            vec.use_torch_stream()
+            for _ in range(3):
+                policy(vec.observations, out=vec.actions)
+                vec.step()
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            vec.use_torch_stream()
+            policy(vec.observations, out=vec.actions)
+            vec.step()
+        torch.cuda.synchronize()
+        t0 = time.perf_counter()
+        for _ in range(a.steps):
+            g.replay()
+        torch.cuda.synchronize()
+        el = time.perf_counter() - t0
+    print(f"drone_amd.policy layers, captured as one hipGraph per step: {a.envs * a.steps / el:.3e} env-steps/s ({el * 1e6 / a.steps:.1f} us per step)")
+    del g
+
+    # act, learn, update: collect K steps (Drone.collect), move the actions along their advantage over the batch's mean
+    # reward, one optimizer step (clip + AdamW of all tensors)
+    vec.use_torch_stream()
+    opt = AdamW(policy.parameters(), lr=3e-4, max_grad_norm=0.5)
+    noise = torch.Generator(device=dev).manual_seed(0)
+
+    def explore(obs, out):
+        policy(obs, out=out)
+        out.add_(torch.randn(out.shape, device=dev, generator=noise), alpha=0.1)
+
+    torch.cuda.synchronize()
+    t0 = time.perf_counter()
+    updates = max(1, a.steps // (10 * K))
+    for _ in range(updates):
+        obs, act, rew, *_ = env.collect(explore, K)
+        advantage = (rew - rew.mean()).unsqueeze(-1)
+        loss = (advantage * (policy(obs) - act).square()).sum(-1).mean()
+        opt.zero_grad()
+        loss.backward()
+        opt.step()
+    torch.cuda.synchronize()
+    el = time.perf_counter() - t0
+    print(f"act, learn, update: {updates} updates of {K} x {a.envs} rows, {el * 1e6 / updates:.0f} us each; gradient norm {opt.grad_norm[0].item():.3e}")
     env.close()
 
 

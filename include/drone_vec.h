@@ -358,6 +358,96 @@ void* drone_device_malloc(int device, size_t bytes);
 void drone_device_free(int device, void* p);
 int drone_vec_copy_to_host(DroneVec* v, void* host_dst, const void* device_src, size_t bytes);
 
+/* ---- the policy beside the env: its layers, their gradients, the optimizer step ----
+ * For a learner whose observations, policy and gradients stay in HBM next to the env (policy forward -> actions buffer ->
+ * drone_vec_step on one stream). No handle and no state of their own: device pointers and sizes in a struct, a HIP device
+ * ordinal, a stream (hipStream_t as void*, NULL: the device's default stream), a caller-owned workspace where one is
+ * needed. Asynchronous on the stream, capturable into a hipGraph, the caller's current device is put back. 0, or -1 with
+ * drone_last_error(). Pointers must be device memory of `device`; leading dimensions count elements, rows are contiguous.
+ * Results depend on no atomics: the same call gives the same bits. A workspace is scratch of one call: calls that may run
+ * at the same time (two streams, two graphs) need one each. */
+#define DRONE_F32 0
+#define DRONE_BF16 1
+#define DRONE_F16 2
+
+#define DRONE_ACTIVATION_NONE 0
+#define DRONE_ACTIVATION_RELU 1
+#define DRONE_ACTIVATION_TANH 2
+#define DRONE_ACTIVATION_SILU 3
+#define DRONE_ACTIVATION_GELU 4 /* the erf form */
+
+/* y = act(x W^T + b) + residual: one launch. x [rows][in], weight [out][in], bias [out], residual / y [rows][out], all of
+ * `dtype`; products are summed in 32 bits, the result is rounded once. `slope` (forward, or NULL when nothing will be
+ * differentiated) receives act'(z), [rows][out] dense, fp16 for DRONE_BF16 and f32 for the others. Backward reads it
+ * (NULL only for DRONE_ACTIVATION_NONE) with dy [rows][out] and writes those of
+ *   dx = dz W,   dweight = dz^T x,   dbias = sum of dz over the rows,   dz = dy * slope
+ * that are not NULL (dweight [out][in] and dbias [out] dense); the residual's gradient is dy itself. y may be the residual
+ * (same pointer and leading dimension); no other output may overlap an input. rows 0 ... 2^31 - 1 (0: sums are zero),
+ * in / out 1 ... 65536. Backward with dweight or dbias needs drone_linear_workspace bytes at `workspace` (16-byte aligned). */
+typedef struct DroneLinear {
+    uint32_t struct_size; /* = sizeof(DroneLinear) */
+    int32_t device, dtype, activation;
+    int64_t rows, in_features, out_features;
+    const void *x, *weight, *bias, *residual, *dy;
+    void *y, *slope, *dx, *dweight, *dbias;
+    int64_t x_ld, weight_ld, residual_ld, dy_ld, y_ld, dx_ld;
+    void* workspace;
+    uint64_t workspace_bytes;
+} DroneLinear;
+int drone_linear_forward(const DroneLinear* call, void* hip_stream);
+int drone_linear_backward(const DroneLinear* call, void* hip_stream);
+uint64_t drone_linear_workspace(const DroneLinear* call); /* bytes drone_linear_backward needs; 0 with drone_last_error() if the call is wrong */
+
+/* The norms after and before a residual block, fused with the block's gate and residual scale:
+ *   r = x + scale * sigmoid(gate) * (n(block) * post_weight);   h = n(r) * pre_weight;   n(a) = a / sqrt(mean(a^2) + eps)
+ * x, block, r, h [rows][width] of `dtype`; weights [width] or NULL (ones); block NULL: r = x; gate_kind 0: none, 1: one
+ * [width] for every row, 2: [rows][width]. r may be NULL. Everything between is 32-bit, r and h are rounded once (h from
+ * the unrounded r). Backward takes the same inputs and dr, dh (either may be NULL: zero) and writes those of dx, dblock,
+ * dgate ([width] or [rows][width] by gate_kind), dpost_weight, dpre_weight that are not NULL. r, h, dr, dh and the
+ * gradients are dense. width 1 ... 4096; drone_norm_workspace bytes for the [width] gradients. No output may overlap an input. */
+typedef struct DroneNorm {
+    uint32_t struct_size; /* = sizeof(DroneNorm) */
+    int32_t device, dtype, gate_kind;
+    int64_t rows, width;
+    const void *x, *block, *gate, *post_weight, *pre_weight, *dr, *dh;
+    void *r, *h, *dx, *dblock, *dgate, *dpost_weight, *dpre_weight;
+    int64_t x_ld, block_ld, gate_ld;
+    float scale, eps;
+    void* workspace;
+    uint64_t workspace_bytes;
+} DroneNorm;
+int drone_norm_forward(const DroneNorm* call, void* hip_stream);
+int drone_norm_backward(const DroneNorm* call, void* hip_stream);
+uint64_t drone_norm_workspace(const DroneNorm* call);
+
+/* One AdamW step over `count` tensors, clipped by the global norm of their gradients:
+ *   c = min(1, max_grad_norm / (sqrt(sum g^2) + 1e-6)) (1 if max_grad_norm <= 0);  g' = c g
+ *   m = beta1 m + (1 - beta1) g';  v = beta2 v + (1 - beta2) g'^2
+ *   p = p (1 - lr weight_decay) - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps)
+ * p and g of `dtype`, m and v f32, master f32 (required for the 16-bit types, whose p is the rounded master; NULL for
+ * DRONE_F32), each dense with `elements` values. `step` (device, one int32) counts the steps done: the call adds 1 and t is
+ * the result, so a captured call replays with an advancing t (lr and the rest stay those of the capture). `grad_norm`
+ * (device, one f32) or NULL receives the norm before clipping. `tensors` is host memory, read during the call. No tensor
+ * may appear twice. drone_adamw_workspace bytes at `workspace`. */
+typedef struct DroneAdamWTensor {
+    void* param;
+    const void* grad;
+    float *exp_avg, *exp_avg_sq, *master;
+    int64_t elements;
+} DroneAdamWTensor;
+typedef struct DroneAdamW {
+    uint32_t struct_size; /* = sizeof(DroneAdamW) */
+    int32_t device, dtype, count;
+    const DroneAdamWTensor* tensors;
+    int32_t* step;
+    float* grad_norm;
+    double lr, beta1, beta2, eps, weight_decay, max_grad_norm;
+    void* workspace;
+    uint64_t workspace_bytes;
+} DroneAdamW;
+int drone_adamw_step(const DroneAdamW* call, void* hip_stream);
+uint64_t drone_adamw_workspace(const DroneAdamW* call);
+
 /* HIP-event timer on the handle's stream: start, ..launches.., stop → ms. */
 int drone_vec_timer_start(DroneVec* v);
 int drone_vec_timer_stop(DroneVec* v, float* elapsed_ms);
