@@ -5,6 +5,8 @@
 //   weight   DW[n][k] = sum_m DZ[m][n] X[m][k]     split over m, partial sums joined in a fixed order; db rides along
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "drone_policy.hpp"
 
 #include "../../include/drone_vec.h"
@@ -12,14 +14,15 @@
 namespace drone {
 namespace {
 
-constexpr int kThreads = 256;
 constexpr int kPieces = 8;  // 16-byte pieces of the reduction axis a tile row holds: 64 16-bit or 32 f32 elements
+constexpr int kJoinThreads = 256;
 
 template <class T> __device__ __forceinline__ float to_f(T v) { return (float)v; }
 
-// ---- activation: value and slope in 32 bits. PRECISE (f32 tensors): the math library's functions. 16-bit tensors: the
-// hardware exp2 / rcp (1 ulp) are far below the result's own rounding, and erf is Abramowitz & Stegun 7.1.26
-// (|error| <= 1.5e-7), whose exp(-z^2/2) is also what the slope needs. ----
+// ---- activation: value and slope in 32 bits, by the hardware's exp2 and rcp (1 ulp each). tanh and silu keep a relative
+// error of about 1e-6 everywhere (tanh by its series near zero, its slope from 1 - |a|, not from 1 - a^2). erf: the math
+// library's for f32 tensors; Abramowitz & Stegun 7.1.26 (|error| <= 1.5e-7) for the 16-bit types, whose exp(-z^2/2) is
+// also what the slope needs. ----
 template <bool PRECISE>
 __device__ __forceinline__ float activate(float z, int act, float& slope) {
     switch (act) {
@@ -27,19 +30,15 @@ __device__ __forceinline__ float activate(float z, int act, float& slope) {
             slope = z > 0.f ? 1.f : 0.f;
             return z > 0.f ? z : (z != z ? z : 0.f);  // a NaN stays one
         case DRONE_ACTIVATION_TANH: {
-            float a;
-            if (PRECISE) {
-                a = tanhf(z);
-            } else {
-                const float big = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __expf(2.f * z));
-                const float small = z * (1.f - z * z * 0.33333334f);
-                a = fabsf(z) < 0.03f ? small : big;
-            }
-            slope = 1.f - a * a;
-            return a;
+            const float x = 2.f * __builtin_amdgcn_rcpf(1.f + __expf(2.f * fabsf(z)));  // 1 - |tanh z|
+            const float q = z * z;
+            const float series = z * (1.f + q * (-0.33333334f + q * (0.13333334f + q * (-0.05396825f + q * 0.02186949f))));
+            const bool small = q < 0.0625f;  // the series' next term is 1e-8 of z there
+            slope = small ? 1.f - series * series : x * (2.f - x);
+            return small ? series : copysignf(1.f - x, z);
         }
         case DRONE_ACTIVATION_SILU: {
-            const float s = PRECISE ? 1.f / (1.f + expf(-z)) : __builtin_amdgcn_rcpf(1.f + __expf(-z));
+            const float s = __builtin_amdgcn_rcpf(1.f + __expf(-z));
             slope = s * (1.f + z * (1.f - s));
             if (fabsf(z) > 80.f) {  // 0 * inf at the infinities: the limits instead
                 slope = z > 0.f ? 1.f : 0.f;
@@ -48,7 +47,7 @@ __device__ __forceinline__ float activate(float z, int act, float& slope) {
             return z * s;
         }
         case DRONE_ACTIVATION_GELU: {
-            const float e = PRECISE ? expf(-0.5f * z * z) : __expf(-0.5f * z * z);
+            const float e = __expf(-0.5f * z * z);
             float cdf;
             if (PRECISE) {
                 cdf = 0.5f * (1.f + erff(z * 0.70710678f));
@@ -73,113 +72,132 @@ __device__ __forceinline__ float activate(float z, int act, float& slope) {
     }
 }
 
+// ---- memory: N elements at any element-aligned address. The vector accesses of gfx950 take unaligned global addresses, so
+// rows of 333 halves move in 16-byte pieces like rows of 336, and only a row's last piece goes element by element ----
+template <class S, int N> struct Vec { S e[N]; };
+
+template <class S, int N>
+__device__ __forceinline__ Vec<S, N> load_n(const S* p, long long left) {
+    Vec<S, N> v;
+    if (left >= N) {
+        __builtin_memcpy(&v, p, sizeof(v));
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; e++) v.e[e] = (S)0.f;
+#pragma unroll
+        for (int e = 0; e < N; e++) if (e < left) v.e[e] = p[e];
+    }
+    return v;
+}
+
+template <class S, int N>
+__device__ __forceinline__ void store_n(S* p, long long left, const float* f) {
+    Vec<S, N> v;
+#pragma unroll
+    for (int e = 0; e < N; e++) v.e[e] = (S)f[e];
+    if (left >= N) {
+        __builtin_memcpy(p, &v, sizeof(v));
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; e++) if (e < left) p[e] = v.e[e];
+    }
+}
+
 // ---- tiles in LDS: [row][8 pieces of 16 B], piece p of row r at p ^ swz(r): eight neighbouring rows read the same piece
 // from eight different bank groups, and the transposing loader's lanes (four rows apart) write to eight as well ----
 __device__ __forceinline__ int swz(int r) { return (r ^ (r >> 3)) & 7; }
 
-template <class T>
-__device__ __forceinline__ u32x4 pack(const float* f) {
-    union { u32x4 u; T t[Elem<T>::kE]; } o;
-#pragma unroll
-    for (int e = 0; e < Elem<T>::kE; e++) o.t[e] = (T)f[e];
-    return o.u;
-}
+// The matrix instruction leaves a lane the result rows 8 a + 4 half + b (a, b = 0 ... 3) of its first operand. The features
+// are that operand, and feature 16 half + 4 a + b of every 32 is put into that row, so a lane owns 16 neighbouring features
+// of one output row: 32- or 64-byte pieces instead of 8- or 16-byte ones.
+__device__ __forceinline__ int feature_of(int i) { return (i & ~31) | ((i & 4) << 2) | ((i & 24) >> 1) | (i & 3); }
+__device__ __forceinline__ int row_of_feature(int f) { return (f & ~31) | ((f & 16) >> 2) | ((f & 12) << 1) | (f & 3); }
 
-// One operand as it lies in memory. CONTIG: [row][reduction]; otherwise [reduction][row]. With `slope` the element is
-// v * slope (the dz of the gradient), formed in 32 bits and rounded once to T for the matrix core.
+// One operand as it lies in memory. CONTIG tiles: [row][reduction]; the others: [reduction][row]. With `slope` (a dense
+// companion) the element is v * slope: the dz of the gradient, formed in 32 bits and rounded once for the matrix core.
 template <class T>
 struct Operand {
     const T* p;
     long long ld;
-    const typename Elem<T>::Slope* slope;  // dense companion with leading dimension slope_ld, or null
+    const typename Elem<T>::Slope* slope;
     long long slope_ld;
 };
 
-// Loads ROWS x 8 pieces of a [row][reduction] operand: thread t takes piece t % 8 of rows t / 8 + 32 i.
-template <class T, int ROWS, bool VEC>
+// Holds ROWS x 8 pieces of a [row][reduction] operand: thread t takes piece t % 8 of rows t / 8 + i THREADS / 8. Rows past
+// the end repeat the last one (their results are not stored), the reduction past its end is zero.
+template <class T, int ROWS, int THREADS, bool FEATURES>
 struct ContigTile {
-    static constexpr int kE = Elem<T>::kE, kN = ROWS * kPieces / kThreads;
-    u32x4 reg[kN];
+    static constexpr int kE = Elem<T>::kE, kN = ROWS * kPieces / THREADS;
+    Vec<T, kE> reg[kN];
+    static __device__ __forceinline__ int lds_row(int i) { return (threadIdx.x >> 3) + i * (THREADS / 8); }
     __device__ __forceinline__ void load(const Operand<T>& o, long long row0, long long rows, long long k0, long long kend) {
-        const int t = threadIdx.x, c = t & 7;
-        const long long k = k0 + c * kE;
+        if (k0 + kPieces * kE <= kend) some<true>(o, row0, rows, k0, kend); else some<false>(o, row0, rows, k0, kend);
+    }
+    // WHOLE: no piece of the tile crosses the end (the same for the workgroup), so the loads go out without a branch between
+    template <bool WHOLE>
+    __device__ __forceinline__ void some(const Operand<T>& o, long long row0, long long rows, long long k0, long long kend) {
+        const long long k = k0 + (threadIdx.x & 7) * kE, left = WHOLE ? kE : kend - k;
 #pragma unroll
         for (int i = 0; i < kN; i++) {
-            const long long r = row0 + (t >> 3) + i * (kThreads / 8);
-            union { u32x4 u; T e[kE]; } v;
-            v.u = u32x4{0, 0, 0, 0};
-            if (r < rows && k < kend) {
-                const T* p = o.p + r * o.ld + k;
-                if (VEC) {
-                    v.u = *(const u32x4*)p;
-                } else {
+            long long r = row0 + (FEATURES ? feature_of(lds_row(i)) : lds_row(i));
+            r = r < rows ? r : rows - 1;
+            if (left <= 0) {
 #pragma unroll
-                    for (int e = 0; e < kE; e++) if (k + e < kend) v.e[e] = p[e];
-                }
-                if (o.slope) {
-                    const auto* q = o.slope + r * o.slope_ld + k;
-                    float f[kE];
-                    if (VEC) {
-                        struct Slopes { typename Elem<T>::Slope e[kE]; };
-                        const Slopes s = *(const Slopes*)__builtin_assume_aligned(q, 16);
-#pragma unroll
-                        for (int e = 0; e < kE; e++) f[e] = to_f(v.e[e]) * to_f(s.e[e]);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < kE; e++) f[e] = k + e < kend ? to_f(v.e[e]) * to_f(q[e]) : 0.f;
-                    }
-                    v.u = pack<T>(f);
-                }
+                for (int e = 0; e < kE; e++) reg[i].e[e] = (T)0.f;
+                continue;
             }
-            reg[i] = v.u;
+            reg[i] = load_n<T, kE>(o.p + r * o.ld + k, left);
+            if (o.slope) {
+                const auto q = load_n<typename Elem<T>::Slope, kE>(o.slope + r * o.slope_ld + k, left);
+#pragma unroll
+                for (int e = 0; e < kE; e++) reg[i].e[e] = (T)(to_f(reg[i].e[e]) * to_f(q.e[e]));
+            }
         }
     }
     __device__ __forceinline__ void store(u32x4* lds) const {
-        const int t = threadIdx.x, c = t & 7;
 #pragma unroll
         for (int i = 0; i < kN; i++) {
-            const int r = (t >> 3) + i * (kThreads / 8);
-            lds[r * kPieces + (c ^ swz(r))] = reg[i];
+            const int r = lds_row(i);
+            lds[r * kPieces + ((threadIdx.x & 7) ^ swz(r))] = __builtin_bit_cast(u32x4, reg[i]);
         }
     }
 };
 
-// Loads the same tile from a [reduction][row] operand: a thread takes kE reduction steps x 4 rows (kE loads of 4 elements)
+// Holds the same tile from a [reduction][row] operand: a thread takes kE reduction steps x 4 rows (kE loads of 4 elements)
 // and turns them in registers, so the LDS tile and the fragment reads are those of the contiguous form.
-template <class T, int ROWS, bool VEC>
+template <class T, int ROWS, int THREADS, bool FEATURES>
 struct TransTile {
-    static constexpr int kE = Elem<T>::kE, kBlocks = ROWS / 4 * kPieces, kN = (kBlocks + kThreads - 1) / kThreads;
-    struct Four { T e[4]; } reg[kN][kE];
+    static constexpr int kE = Elem<T>::kE, kBlocks = ROWS / 4 * kPieces, kN = (kBlocks + THREADS - 1) / THREADS;
+    Vec<T, 4> reg[kN][kE];
     // add: the 32-bit dz of this thread's four rows is added up over the reduction (the bias gradient)
     __device__ __forceinline__ void load(const Operand<T>& o, long long row0, long long rows, long long k0, long long kend, bool add, float (&sum)[kN][4]) {
+        if (k0 + kPieces * kE <= kend && row0 + ROWS <= rows) some<true>(o, row0, rows, k0, kend, add, sum); else some<false>(o, row0, rows, k0, kend, add, sum);
+    }
+    template <bool WHOLE>
+    __device__ __forceinline__ void some(const Operand<T>& o, long long row0, long long rows, long long k0, long long kend, bool add, float (&sum)[kN][4]) {
 #pragma unroll
         for (int i = 0; i < kN; i++) {
-            const int b = threadIdx.x + i * kThreads;
-            const long long r = row0 + (b % (ROWS / 4)) * 4, k = k0 + b / (ROWS / 4) * kE;
+            const int b = threadIdx.x + i * THREADS;
+            const long long r = row0 + (b % (ROWS / 4)) * 4, k = k0 + b / (ROWS / 4) * kE, left = WHOLE ? 4 : rows - r;
+            const bool mine = kBlocks % THREADS == 0 || b < kBlocks;
 #pragma unroll
             for (int e = 0; e < kE; e++) {
-                Four v;
+                Vec<T, 4> v;
 #pragma unroll
                 for (int j = 0; j < 4; j++) v.e[j] = (T)0.f;
-                if (b < kBlocks && k + e < kend && r < rows) {
-                    const T* p = o.p + (k + e) * o.ld + r;
-                    if (VEC) {
-                        v = *(const Four*)__builtin_assume_aligned(p, sizeof(Four));
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 4; j++) if (r + j < rows) v.e[j] = p[j];
-                    }
-                    if (o.slope || add) {
-                        struct S4 { typename Elem<T>::Slope e[4]; } s;
-                        const auto* q = o.slope ? o.slope + (k + e) * o.slope_ld + r : nullptr;
-                        if (VEC && q) s = *(const S4*)__builtin_assume_aligned(q, sizeof(S4));
+                if (mine && (WHOLE || (k + e < kend && left > 0))) {
+                    v = load_n<T, 4>(o.p + (k + e) * o.ld + r, left);
+                    if (o.slope) {
+                        const auto q = load_n<typename Elem<T>::Slope, 4>(o.slope + (k + e) * o.slope_ld + r, left);
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
-                            float f = to_f(v.e[j]);
-                            if (q) f *= VEC ? to_f(s.e[j]) : (r + j < rows ? to_f(q[j]) : 0.f);
+                            const float f = to_f(v.e[j]) * to_f(q.e[j]);
                             if (add) sum[i][j] += f;
                             v.e[j] = (T)f;
                         }
+                    } else if (add) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) sum[i][j] += to_f(v.e[j]);
                     }
                 }
                 reg[i][e] = v;
@@ -189,15 +207,15 @@ struct TransTile {
     __device__ __forceinline__ void store(u32x4* lds) const {
 #pragma unroll
         for (int i = 0; i < kN; i++) {
-            const int b = threadIdx.x + i * kThreads;
-            if (b >= kBlocks) break;
-            const int r = (b % (ROWS / 4)) * 4, c = b / (ROWS / 4);
+            const int b = threadIdx.x + i * THREADS;
+            if (kBlocks % THREADS && b >= kBlocks) break;
+            const int r = (b % (ROWS / 4)) * 4, c = b / (ROWS / 4), at = FEATURES ? row_of_feature(r) : r;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                union { u32x4 u; T t[kE]; } v;
+                Vec<T, kE> v;
 #pragma unroll
-                for (int e = 0; e < kE; e++) v.t[e] = reg[i][e].e[j];
-                lds[(r + j) * kPieces + (c ^ swz(r + j))] = v.u;
+                for (int e = 0; e < kE; e++) v.e[e] = reg[i][e].e[j];
+                lds[(at + j) * kPieces + (c ^ swz(at + j))] = __builtin_bit_cast(u32x4, v);
             }
         }
     }
@@ -218,51 +236,33 @@ __device__ __forceinline__ void mfma(f32x16& d, const u32x4& a, const u32x4& b, 
 
 enum Product { kForward, kInput, kWeight };
 
-template <class T, int ROWS, bool CONTIG, bool VEC> struct TileOf { using type = ContigTile<T, ROWS, VEC>; };
-template <class T, int ROWS, bool VEC> struct TileOf<T, ROWS, false, VEC> { using type = TransTile<T, ROWS, VEC>; };
+template <class T, int ROWS, int THREADS, bool CONTIG, bool FEATURES> struct TileOf { using type = ContigTile<T, ROWS, THREADS, FEATURES>; };
+template <class T, int ROWS, int THREADS, bool FEATURES> struct TileOf<T, ROWS, THREADS, false, FEATURES> { using type = TransTile<T, ROWS, THREADS, FEATURES>; };
 
-template <class S> struct FourOf { S e[4]; };
-
-template <class S>
-__device__ __forceinline__ void load4(const S* p, int left, bool vec, float* f) {
-    if (vec) {
-        const FourOf<S> v = *(const FourOf<S>*)__builtin_assume_aligned(p, sizeof(FourOf<S>));
-#pragma unroll
-        for (int j = 0; j < 4; j++) f[j] = to_f(v.e[j]);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; j++) f[j] = j < left ? to_f(p[j]) : 0.f;
-    }
+// A unit of work: one output tile of one part of the reduction. Units go to the XCDs in eight contiguous ranges (workgroups
+// go round the XCDs), parts outermost, feature tiles innermost: workgroups that read the same rows share an L2.
+struct Unit { long long part, tm; int tn; bool none; };
+__device__ __forceinline__ Unit unit_of(long long tiles, int tiles_n, long long units) {
+    const long long per = (units + 7) / 8, u = (long long)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    Unit r;
+    r.none = (long long)(blockIdx.x >> 3) >= per || u >= units;
+    r.part = u / tiles;
+    const long long tile = u - r.part * tiles;
+    r.tm = tile / tiles_n;
+    r.tn = (int)(tile - r.tm * tiles_n);
+    return r;
 }
 
-template <class S>
-__device__ __forceinline__ void store4(S* p, int left, bool vec, const float* f) {
-    if (vec) {
-        FourOf<S> v;
-#pragma unroll
-        for (int j = 0; j < 4; j++) v.e[j] = (S)f[j];
-        *(FourOf<S>*)__builtin_assume_aligned(p, sizeof(FourOf<S>)) = v;
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; j++) if (j < left) p[j] = (S)f[j];
-    }
-}
-
-// BM x BN outputs a workgroup (rows x features), four waves WM x WN. The features are the matrix instruction's first
-// operand, so a lane ends up with four neighbouring features of one row.
-template <class T, Product P, bool VEC, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(kThreads) void linear_kernel(LinearArgs a, int tiles_n, long long tiles, long long red_part, int out_vec) {
+// BM x BN outputs a workgroup (rows x features), WM x WN waves.
+template <class T, Product P, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64) void linear_kernel(LinearArgs a, int tiles_n, long long tiles, int parts, long long red_part) {
     using Slope = typename Elem<T>::Slope;
-    constexpr int kE = Elem<T>::kE, kK = kPieces * kE, TM = BM / WM / 32, TN = BN / WN / 32;
-    static_assert(WM * WN * 64 == kThreads && TM >= 1 && TN >= 1, "four waves");
+    constexpr int kThreads = WM * WN * 64, kE = Elem<T>::kE, kK = kPieces * kE, TM = BM / WM / 32, TN = BN / WN / 32;
+    static_assert(TM >= 1 && TN >= 1 && BM % (kThreads / 8) == 0 && BN % (kThreads / 8) == 0, "a whole number of pieces for each thread");
     __shared__ u32x4 lds[2][(BM + BN) * kPieces];
 
-    // tile number: one contiguous eighth of the tiles per XCD (workgroups go round the eight XCDs), features fastest, so
-    // the workgroups that share a row tile share its L2
-    const long long per = (tiles + 7) / 8, tile = (long long)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if ((blockIdx.x >> 3) >= per || tile >= tiles) return;
-    const long long tm = tile / tiles_n;
-    const int tn = (int)(tile - tm * tiles_n);
+    const Unit unit = unit_of(tiles, tiles_n, tiles * parts);
+    if (unit.none) return;
 
     Operand<T> rowsop, featop;
     long long nrows, nfeat, red0 = 0, red1;
@@ -279,16 +279,16 @@ __global__ __launch_bounds__(kThreads) void linear_kernel(LinearArgs a, int tile
         rowsop = {(const T*)a.dy, a.dy_ld, slope, a.out};
         featop = {(const T*)a.x, a.x_ld, nullptr, 0};
         nrows = a.out; nfeat = a.in;
-        red0 = (long long)blockIdx.y * red_part;
+        red0 = unit.part * red_part;
         red1 = red0 + red_part < a.rows ? red0 + red_part : a.rows;
     }
-    const long long row0 = tm * BM, feat0 = (long long)tn * BN;
+    const long long row0 = unit.tm * BM, feat0 = (long long)unit.tn * BN;
 
-    typename TileOf<T, BM, P != kWeight, VEC>::type rt;
-    typename TileOf<T, BN, P == kForward, VEC>::type ft;
+    typename TileOf<T, BM, kThreads, P != kWeight, false>::type rt;
+    typename TileOf<T, BN, kThreads, P == kForward, true>::type ft;
     constexpr int kSums = (BM / 4 * kPieces + kThreads - 1) / kThreads, kNoSums = (BN / 4 * kPieces + kThreads - 1) / kThreads;
     float sum[kSums][4] = {}, no_sum[kNoSums][4];
-    const bool want_db = P == kWeight && a.db && tn == 0;
+    const bool want_db = P == kWeight && a.db && unit.tn == 0;
     auto fetch = [&](long long k) {
         if constexpr (P == kWeight) rt.load(rowsop, row0, nrows, k, red1, want_db, sum); else rt.load(rowsop, row0, nrows, k, red1);
         if constexpr (P == kForward) ft.load(featop, feat0, nfeat, k, red1); else ft.load(featop, feat0, nfeat, k, red1, false, no_sum);
@@ -322,39 +322,46 @@ __global__ __launch_bounds__(kThreads) void linear_kernel(LinearArgs a, int tile
         buf ^= 1;  // the next store goes to the other buffer; the barrier behind it says that everyone has left this one
     }
 
+    auto epilogue = [&](auto whole) {
+        constexpr bool kWhole = decltype(whole)::value;
 #pragma unroll
-    for (int m = 0; m < TM; m++) {
-        const long long row = row0 + wrow + m * 32 + l32;
-        if (row >= nrows) continue;
+        for (int m = 0; m < TM; m++) {
+            const long long row = row0 + wrow + m * 32 + l32;
+            if (row >= nrows) continue;
 #pragma unroll
-        for (int n = 0; n < TN; n++)
+            for (int n = 0; n < TN; n++)
 #pragma unroll
-            for (int q = 0; q < 4; q++) {  // register 4 q + j of a lane: feature 8 q + 4 half + j
-                const long long feat = feat0 + wfeat + n * 32 + q * 8 + half * 4;
-                if (feat >= nfeat) continue;
-                const int left = nfeat - feat < 4 ? (int)(nfeat - feat) : 4;
-                float v[4];
+                for (int q = 0; q < 16 / kE; q++) {  // register r of a lane: feature 16 half + r
+                    const long long feat = feat0 + wfeat + n * 32 + half * 16 + q * kE, left = kWhole ? kE : nfeat - feat;
+                    if (left <= 0) continue;
+                    float v[kE];
 #pragma unroll
-                for (int j = 0; j < 4; j++) v[j] = acc[n][m][4 * q + j];
-                if (P == kForward) {
-                    float b[4] = {0.f, 0.f, 0.f, 0.f}, s[4];
-                    if (a.b) load4((const T*)a.b + feat, left, out_vec, b);
+                    for (int j = 0; j < kE; j++) v[j] = acc[n][m][kE * q + j];
+                    if (P == kForward) {
+                        float s[kE];
+                        if (a.b) {
+                            const auto b = load_n<T, kE>((const T*)a.b + feat, left);
 #pragma unroll
-                    for (int j = 0; j < 4; j++) v[j] = activate<sizeof(T) == 4>(v[j] + b[j], a.act, s[j]);
-                    if (a.slope) store4((Slope*)a.slope + row * a.out + feat, left, out_vec, s);
-                    if (a.res) {
-                        load4((const T*)a.res + row * a.res_ld + feat, left, out_vec, b);
+                            for (int j = 0; j < kE; j++) v[j] += to_f(b.e[j]);
+                        }
 #pragma unroll
-                        for (int j = 0; j < 4; j++) v[j] += b[j];
+                        for (int j = 0; j < kE; j++) v[j] = activate<sizeof(T) == 4>(v[j], a.act, s[j]);
+                        if (a.slope) store_n<Slope, kE>((Slope*)a.slope + row * a.out + feat, left, s);
+                        if (a.res) {
+                            const auto b = load_n<T, kE>((const T*)a.res + row * a.res_ld + feat, left);
+#pragma unroll
+                            for (int j = 0; j < kE; j++) v[j] += to_f(b.e[j]);
+                        }
+                        store_n<T, kE>((T*)a.y + row * a.y_ld + feat, left, v);
+                    } else if (P == kInput) {
+                        store_n<T, kE>((T*)a.dx + row * a.dx_ld + feat, left, v);
+                    } else {
+                        store_n<float, kE>(a.work + unit.part * a.out * a.in + row * a.in + feat, left, v);
                     }
-                    store4((T*)a.y + row * a.y_ld + feat, left, out_vec, v);
-                } else if (P == kInput) {
-                    store4((T*)a.dx + row * a.dx_ld + feat, left, out_vec, v);
-                } else {
-                    store4(a.work + (long long)blockIdx.y * a.out * a.in + row * a.in + feat, left, out_vec, v);
                 }
-            }
-    }
+        }
+    };
+    if (feat0 + BN <= nfeat) epilogue(std::true_type{}); else epilogue(std::false_type{});
     if constexpr (P == kWeight) {
         if (want_db) {  // threads of one row group hold the sums of eight reduction pieces: joined in order through LDS
             float* join = (float*)lds;
@@ -367,110 +374,96 @@ __global__ __launch_bounds__(kThreads) void linear_kernel(LinearArgs a, int tile
                     for (int j = 0; j < 4; j++) join[(b / (BM / 4)) * BM + (b % (BM / 4)) * 4 + j] = sum[i][j];
             }
             __syncthreads();
-            if (threadIdx.x < BM && row0 + threadIdx.x < nrows) {
+            for (int i = threadIdx.x; i < BM && row0 + i < nrows; i += kThreads) {
                 float s = 0.f;
 #pragma unroll
-                for (int c = 0; c < kPieces; c++) s += join[c * BM + threadIdx.x];
-                a.work[(long long)gridDim.y * a.out * a.in + (long long)blockIdx.y * a.out + row0 + threadIdx.x] = s;
+                for (int c = 0; c < kPieces; c++) s += join[c * BM + i];
+                a.work[(long long)parts * a.out * a.in + unit.part * a.out + row0 + i] = s;
             }
         }
     }
 }
 
-// Joins the partial sums of the weight and bias gradients, part by part in order: every result is the same in every run.
+// Joins the partial sums of the weight and bias gradients in a fixed order, 32 values a workgroup, eight threads a value:
+// every result is the same in every run.
 template <class T>
-__global__ __launch_bounds__(kThreads) void linear_join_kernel(const float* work, T* dw, T* db, long long weights, int out, int parts) {
-    const long long i = (long long)blockIdx.x * kThreads + threadIdx.x;
-    const long long all = (dw ? weights : 0) + (db ? out : 0);
-    if (i >= all) return;
-    const bool is_w = dw && i < weights;
-    const long long at = is_w ? i : i - (dw ? weights : 0), step = is_w ? weights : out;
+__global__ __launch_bounds__(kJoinThreads) void linear_join_kernel(const float* work, T* dw, T* db, long long weights, int out, int parts) {
+    __shared__ float join[8][32];
+    const int c = threadIdx.x & 31, slice = threadIdx.x >> 5;
+    const long long i = (long long)blockIdx.x * 32 + c, nw = dw ? weights : 0, all = nw + (db ? out : 0);
+    const bool is_w = i < nw;
+    const long long at = is_w ? i : i - nw, step = is_w ? weights : out;
     const float* p = is_w ? work + at : work + parts * weights + at;
     float s = 0.f;
-    for (int k = 0; k < parts; k++) s += p[k * step];
+    if (i < all)
+#pragma unroll 4
+        for (int k = slice; k < parts; k += 8) s += p[k * step];
+    join[slice][c] = s;
+    __syncthreads();
+    if (slice || i >= all) return;
+#pragma unroll
+    for (int k = 1; k < 8; k++) s += join[k][c];
     if (is_w) dw[at] = (T)s; else db[at] = (T)s;
 }
 
-bool aligned(const void* p, size_t bytes) { return ((uintptr_t)p % bytes) == 0; }
-
-// Parts the weight gradient's reduction is split into: enough workgroups to fill the 256 CUs twice, at least 256 rows each.
-int weight_parts(long long rows, int in, int out, int bm, int bn) {
-    const long long tiles = (long long)((out + bm - 1) / bm) * ((in + bn - 1) / bn);
-    long long parts = (512 + tiles - 1) / tiles, most = (rows + 255) / 256;
-    if (parts > most) parts = most;
-    return parts < 1 ? 1 : (int)parts;
-}
-
-int tile_of(long long n) { return n <= 32 ? 32 : n <= 64 ? 64 : 128; }
-
-template <class T, Product P, bool VEC, int BM, int BN, int WM, int WN>
-int launch(const LinearArgs& a, long long nrows, long long nfeat, int parts, long long red_part, int out_vec, hipStream_t s) {
+template <class T, Product P, int BM, int BN, int WM, int WN>
+int launch(const LinearArgs& a, long long nrows, long long nfeat, int parts, long long red_part, hipStream_t s) {
     const int tiles_n = (int)((nfeat + BN - 1) / BN);
-    const long long tiles = (nrows + BM - 1) / BM * tiles_n;
-    const dim3 grid((unsigned)((tiles + 7) / 8 * 8), (unsigned)parts);
-    linear_kernel<T, P, VEC, BM, BN, WM, WN><<<grid, kThreads, 0, s>>>(a, tiles_n, tiles, red_part, out_vec);
+    const long long tiles = (nrows + BM - 1) / BM * tiles_n, units = tiles * parts;
+    linear_kernel<T, P, BM, BN, WM, WN><<<(unsigned)((units + 7) / 8 * 8), WM * WN * 64, 0, s>>>(a, tiles_n, tiles, parts, red_part);
     return (int)hipGetLastError();
 }
 
-template <class T, bool VEC>
-int forward(const LinearArgs& a, int out_vec, hipStream_t s) {
-    switch (tile_of(a.out)) {
-        case 32: return launch<T, kForward, VEC, 128, 32, 4, 1>(a, a.rows, a.out, 1, 0, out_vec, s);
-        case 64: return launch<T, kForward, VEC, 128, 64, 4, 1>(a, a.rows, a.out, 1, 0, out_vec, s);
-        default: return launch<T, kForward, VEC, 128, 128, 2, 2>(a, a.rows, a.out, 1, 0, out_vec, s);
+// Few rows: 32-row tiles, so that 1 024 envs make 32 workgroups and not 8.
+bool few(long long rows, long long feats) { return (rows + 127) / 128 * ((feats + 127) / 128) < 128; }
+
+template <class T, Product P>
+int product(const LinearArgs& a, long long feats, hipStream_t s) {
+    if (few(a.rows, feats)) {
+        if (feats <= 32) return launch<T, P, 32, 32, 1, 1>(a, a.rows, feats, 1, 0, s);
+        return launch<T, P, 32, 64, 1, 2>(a, a.rows, feats, 1, 0, s);
     }
+    if (feats <= 32) return launch<T, P, 128, 32, 4, 1>(a, a.rows, feats, 1, 0, s);
+    if (feats <= 64) return launch<T, P, 128, 64, 4, 1>(a, a.rows, feats, 1, 0, s);
+    return launch<T, P, 128, 128, 2, 2>(a, a.rows, feats, 1, 0, s);
 }
 
-template <class T, bool VEC>
-int input_grad(const LinearArgs& a, int out_vec, hipStream_t s) {
-    switch (tile_of(a.in)) {
-        case 32: return launch<T, kInput, VEC, 128, 32, 4, 1>(a, a.rows, a.in, 1, 0, out_vec, s);
-        case 64: return launch<T, kInput, VEC, 128, 64, 4, 1>(a, a.rows, a.in, 1, 0, out_vec, s);
-        default: return launch<T, kInput, VEC, 128, 128, 2, 2>(a, a.rows, a.in, 1, 0, out_vec, s);
-    }
+// The weight gradient's reduction over the rows is split into parts: enough workgroups to fill the 256 CUs (twice, unless
+// the product is so small that joining the parts costs more than it), at least 256 rows each.
+struct Split { int bm, bn, parts; };
+Split split_of(long long rows, int in, int out) {
+    Split r = {out <= 64 ? 64 : 128, in <= 64 ? 64 : 128, 1};
+    const long long tiles = (long long)((out + r.bm - 1) / r.bm) * ((in + r.bn - 1) / r.bn), want = tiles <= 2 ? 256 : 512;
+    long long parts = (want + tiles - 1) / tiles;
+    const long long most = (rows + 255) / 256;
+    if (parts > most) parts = most;
+    r.parts = parts < 1 ? 1 : (int)parts;
+    return r;
 }
-
-template <class T, bool VEC>
-int weight_grad(const LinearArgs& a, int out_vec, int parts, hipStream_t s) {
-    constexpr int kK = kPieces * Elem<T>::kE;
-    const long long part = ((a.rows + parts - 1) / parts + kK - 1) / kK * kK;
-    const int bm = tile_of(a.out), bn = tile_of(a.in);
-    if (bm <= 64 && bn <= 64) return launch<T, kWeight, VEC, 64, 64, 2, 2>(a, a.out, a.in, parts, part, out_vec, s);
-    if (bm <= 64) return launch<T, kWeight, VEC, 64, 128, 2, 2>(a, a.out, a.in, parts, part, out_vec, s);
-    if (bn <= 64) return launch<T, kWeight, VEC, 128, 64, 2, 2>(a, a.out, a.in, parts, part, out_vec, s);
-    return launch<T, kWeight, VEC, 128, 128, 2, 2>(a, a.out, a.in, parts, part, out_vec, s);
-}
-
-int parts_of(long long rows, int in, int out) { return weight_parts(rows, in, out, tile_of(out) <= 64 ? 64 : 128, tile_of(in) <= 64 ? 64 : 128); }
 
 template <class T>
-int forward_any(const LinearArgs& a, hipStream_t s) {
-    constexpr int kE = Elem<T>::kE;
-    const bool vec = a.in % kE == 0 && a.x_ld % kE == 0 && a.w_ld % kE == 0 && aligned(a.x, 16) && aligned(a.w, 16);
-    const int ov = a.out % 4 == 0 && a.y_ld % 4 == 0 && aligned(a.y, 4 * sizeof(T)) && (!a.b || aligned(a.b, 4 * sizeof(T))) &&
-                   (!a.res || (a.res_ld % 4 == 0 && aligned(a.res, 4 * sizeof(T)))) && (!a.slope || aligned(a.slope, 16));
-    return vec ? forward<T, true>(a, ov, s) : forward<T, false>(a, ov, s);
+int weight_grad(const LinearArgs& a, const Split& sp, hipStream_t s) {
+    constexpr int kK = kPieces * Elem<T>::kE;
+    const long long part = ((a.rows + sp.parts - 1) / sp.parts + kK - 1) / kK * kK;
+    if (sp.bm == 64 && sp.bn == 64) return launch<T, kWeight, 64, 64, 2, 2>(a, a.out, a.in, sp.parts, part, s);
+    if (sp.bm == 64) return launch<T, kWeight, 64, 128, 2, 2>(a, a.out, a.in, sp.parts, part, s);
+    if (sp.bn == 64) return launch<T, kWeight, 128, 64, 2, 2>(a, a.out, a.in, sp.parts, part, s);
+    return launch<T, kWeight, 128, 128, 2, 2>(a, a.out, a.in, sp.parts, part, s);
 }
 
 template <class T>
 int backward_any(const LinearArgs& a, hipStream_t s) {
-    constexpr int kE = Elem<T>::kE;
     int rc = 0;
-    const bool dy16 = a.out % kE == 0 && a.dy_ld % kE == 0 && aligned(a.dy, 16) && (!a.slope || aligned(a.slope, 16));
-    const bool w4 = a.in % 4 == 0 && a.w_ld % 4 == 0 && aligned(a.w, 4 * sizeof(T));
     if (a.dx && a.rows) {
-        const int ov = a.in % 4 == 0 && a.dx_ld % 4 == 0 && aligned(a.dx, 4 * sizeof(T));
-        rc = dy16 && w4 ? input_grad<T, true>(a, ov, s) : input_grad<T, false>(a, ov, s);
+        rc = product<T, kInput>(a, a.in, s);
         if (rc) return rc;
     }
     if (a.dw || a.db) {
-        const bool dy4 = a.out % 4 == 0 && a.dy_ld % 4 == 0 && aligned(a.dy, 4 * sizeof(T)) && (!a.slope || aligned(a.slope, 4 * sizeof(typename Elem<T>::Slope)));
-        const bool x4 = a.in % 4 == 0 && a.x_ld % 4 == 0 && aligned(a.x, 4 * sizeof(T));
-        const int parts = parts_of(a.rows, a.in, a.out);
-        rc = dy4 && x4 ? weight_grad<T, true>(a, a.in % 4 == 0, parts, s) : weight_grad<T, false>(a, a.in % 4 == 0, parts, s);
+        const Split sp = split_of(a.rows, a.in, a.out);
+        rc = weight_grad<T>(a, sp, s);
         if (rc) return rc;
         const long long weights = (long long)a.out * a.in, all = (a.dw ? weights : 0) + (a.db ? a.out : 0);
-        linear_join_kernel<T><<<(unsigned)((all + kThreads - 1) / kThreads), kThreads, 0, s>>>(a.work, (T*)a.dw, (T*)a.db, weights, a.out, parts);
+        linear_join_kernel<T><<<(unsigned)((all + 31) / 32), kJoinThreads, 0, s>>>(a.work, (T*)a.dw, (T*)a.db, weights, a.out, sp.parts);
         rc = (int)hipGetLastError();
     }
     return rc;
@@ -480,13 +473,13 @@ int backward_any(const LinearArgs& a, hipStream_t s) {
 
 int linear_forward_launch(int dtype, const LinearArgs& a, hipStream_t s) {
     if (!a.rows) return 0;
-    return dtype == DRONE_F32 ? forward_any<float>(a, s) : dtype == DRONE_BF16 ? forward_any<__bf16>(a, s) : forward_any<_Float16>(a, s);
+    return dtype == DRONE_F32 ? product<float, kForward>(a, a.out, s) : dtype == DRONE_BF16 ? product<__bf16, kForward>(a, a.out, s) : product<_Float16, kForward>(a, a.out, s);
 }
 int linear_backward_launch(int dtype, const LinearArgs& a, hipStream_t s) {
     return dtype == DRONE_F32 ? backward_any<float>(a, s) : dtype == DRONE_BF16 ? backward_any<__bf16>(a, s) : backward_any<_Float16>(a, s);
 }
 size_t linear_work_bytes(int, long long rows, int in, int out) {
-    return (size_t)parts_of(rows, in, out) * ((size_t)in * out + out) * sizeof(float);
+    return (size_t)split_of(rows, in, out).parts * ((size_t)in * out + out) * sizeof(float);
 }
 
 }  // namespace drone
