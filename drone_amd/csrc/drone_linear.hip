@@ -23,9 +23,9 @@ template <class T> __device__ __forceinline__ float to_f(T v) { return (float)v;
 // error of about 1e-6 everywhere (tanh by its series near zero, its slope from 1 - |a|, not from 1 - a^2). erf: the math
 // library's for f32 tensors; Abramowitz & Stegun 7.1.26 (|error| <= 1.5e-7) for the 16-bit types, whose exp(-z^2/2) is
 // also what the slope needs. ----
-template <bool PRECISE>
-__device__ __forceinline__ float activate(float z, int act, float& slope) {
-    switch (act) {
+template <int ACT, bool PRECISE>
+__device__ __forceinline__ float activate(float z, float& slope) {
+    switch (ACT) {
         case DRONE_ACTIVATION_RELU:
             slope = z > 0.f ? 1.f : 0.f;
             return z > 0.f ? z : (z != z ? z : 0.f);  // a NaN stays one
@@ -253,9 +253,105 @@ __device__ __forceinline__ Unit unit_of(long long tiles, int tiles_n, long long 
     return r;
 }
 
+// What a lane does with its results: 16 neighbouring features of row row0 + 32 m + lane % 32 for each (n, m). Everything the
+// epilogue reads is asked for before the first value is used.
+template <class T, int ACT, int TM, int TN, bool WHOLE>
+__device__ __forceinline__ void write_forward(const LinearArgs& a, const f32x16 (&acc)[TN][TM], long long row0, long long feat0) {
+    using Slope = typename Elem<T>::Slope;
+    constexpr int kE = Elem<T>::kE, kQ = 16 / kE;
+    const int half = (threadIdx.x >> 5) & 1, l32 = threadIdx.x & 31;
+    u32x4 b[TN][kQ], res[TM][TN][kQ];  // as they come: unpacked where they are used
+    using Piece = Vec<T, kE>;
+    auto feat_of = [&](int n, int q) { return feat0 + n * 32 + half * 16 + q * kE; };  // register r of a lane: feature 16 half + r
+    auto left_of = [&](int n, int q) { return WHOLE ? (long long)kE : a.out - feat_of(n, q); };
+#pragma unroll
+    for (int n = 0; n < TN; n++)
+#pragma unroll
+        for (int q = 0; q < kQ; q++) {
+            b[n][q] = u32x4{0, 0, 0, 0};
+            if (a.b && left_of(n, q) > 0) b[n][q] = __builtin_bit_cast(u32x4, load_n<T, kE>((const T*)a.b + feat_of(n, q), left_of(n, q)));
+        }
+    if (a.res)
+#pragma unroll
+        for (int m = 0; m < TM; m++) {
+            long long row = row0 + m * 32 + l32;
+            row = row < a.rows ? row : a.rows - 1;
+#pragma unroll
+            for (int n = 0; n < TN; n++)
+#pragma unroll
+                for (int q = 0; q < kQ; q++)
+                    if (left_of(n, q) > 0) res[m][n][q] = __builtin_bit_cast(u32x4, load_n<T, kE>((const T*)a.res + row * a.res_ld + feat_of(n, q), left_of(n, q)));
+        }
+#pragma unroll
+    for (int m = 0; m < TM; m++) {
+        const long long row = row0 + m * 32 + l32;
+        if (row >= a.rows) continue;
+#pragma unroll
+        for (int n = 0; n < TN; n++)
+#pragma unroll
+            for (int q = 0; q < kQ; q++) {
+                const long long feat = feat_of(n, q), left = left_of(n, q);
+                if (left <= 0) continue;
+                float v[kE], s[kE];
+                const Piece bias = __builtin_bit_cast(Piece, b[n][q]);
+#pragma unroll
+                for (int j = 0; j < kE; j++) v[j] = activate<ACT, sizeof(T) == 4>(acc[n][m][kE * q + j] + to_f(bias.e[j]), s[j]);
+                if (a.slope) store_n<Slope, kE>((Slope*)a.slope + row * a.out + feat, left, s);
+                if (a.res) {
+                    const Piece r = __builtin_bit_cast(Piece, res[m][n][q]);
+#pragma unroll
+                    for (int j = 0; j < kE; j++) v[j] += to_f(r.e[j]);
+                }
+                store_n<T, kE>((T*)a.y + row * a.y_ld + feat, left, v);
+            }
+    }
+}
+
+template <class T, int ACT, int TM, int TN>
+__device__ __forceinline__ void write_forward_any(const LinearArgs& a, const f32x16 (&acc)[TN][TM], long long row0, long long feat0, bool whole) {
+    if (whole) write_forward<T, ACT, TM, TN, true>(a, acc, row0, feat0); else write_forward<T, ACT, TM, TN, false>(a, acc, row0, feat0);
+}
+
+template <class T, Product P, int TM, int TN>
+__device__ __forceinline__ void write_results(const LinearArgs& a, const f32x16 (&acc)[TN][TM], long long row0, long long nrows, long long feat0, long long nfeat, bool whole, long long part) {
+    constexpr int kE = Elem<T>::kE;
+    if constexpr (P == kForward) {
+        switch (a.act) {  // the same for the whole launch: one branch, not one per value
+            case DRONE_ACTIVATION_RELU: write_forward_any<T, DRONE_ACTIVATION_RELU, TM, TN>(a, acc, row0, feat0, whole); break;
+            case DRONE_ACTIVATION_TANH: write_forward_any<T, DRONE_ACTIVATION_TANH, TM, TN>(a, acc, row0, feat0, whole); break;
+            case DRONE_ACTIVATION_SILU: write_forward_any<T, DRONE_ACTIVATION_SILU, TM, TN>(a, acc, row0, feat0, whole); break;
+            case DRONE_ACTIVATION_GELU: write_forward_any<T, DRONE_ACTIVATION_GELU, TM, TN>(a, acc, row0, feat0, whole); break;
+            default: write_forward_any<T, DRONE_ACTIVATION_NONE, TM, TN>(a, acc, row0, feat0, whole);
+        }
+    } else {
+        const int half = (threadIdx.x >> 5) & 1, l32 = threadIdx.x & 31;
+        auto write = [&](auto is_whole) {
+            constexpr bool kWhole = decltype(is_whole)::value;  // no feature group crosses the end: no branch between the accesses
+#pragma unroll
+            for (int m = 0; m < TM; m++) {
+                const long long row = row0 + m * 32 + l32;
+                if (row >= nrows) continue;
+#pragma unroll
+                for (int n = 0; n < TN; n++)
+#pragma unroll
+                    for (int q = 0; q < 16 / kE; q++) {
+                        const long long feat = feat0 + n * 32 + half * 16 + q * kE, left = kWhole ? kE : nfeat - feat;
+                        if (left <= 0) continue;
+                        float v[kE];
+#pragma unroll
+                        for (int j = 0; j < kE; j++) v[j] = acc[n][m][kE * q + j];
+                        if (P == kInput) store_n<T, kE>((T*)a.dx + row * a.dx_ld + feat, left, v);
+                        else store_n<float, kE>(a.work + part * a.out * a.in + row * a.in + feat, left, v);
+                    }
+            }
+        };
+        if (whole) write(std::true_type{}); else write(std::false_type{});
+    }
+}
+
 // BM x BN outputs a workgroup (rows x features), WM x WN waves.
 template <class T, Product P, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * 64) void linear_kernel(LinearArgs a, int tiles_n, long long tiles, int parts, long long red_part) {
+__global__ __launch_bounds__(WM * WN * 64, 2) void linear_kernel(LinearArgs a, int tiles_n, long long tiles, int parts, long long red_part) {
     using Slope = typename Elem<T>::Slope;
     constexpr int kThreads = WM * WN * 64, kE = Elem<T>::kE, kK = kPieces * kE, TM = BM / WM / 32, TN = BN / WN / 32;
     static_assert(TM >= 1 && TN >= 1 && BM % (kThreads / 8) == 0 && BN % (kThreads / 8) == 0, "a whole number of pieces for each thread");
@@ -322,46 +418,7 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_kernel(LinearArgs a, int 
         buf ^= 1;  // the next store goes to the other buffer; the barrier behind it says that everyone has left this one
     }
 
-    auto epilogue = [&](auto whole) {
-        constexpr bool kWhole = decltype(whole)::value;
-#pragma unroll
-        for (int m = 0; m < TM; m++) {
-            const long long row = row0 + wrow + m * 32 + l32;
-            if (row >= nrows) continue;
-#pragma unroll
-            for (int n = 0; n < TN; n++)
-#pragma unroll
-                for (int q = 0; q < 16 / kE; q++) {  // register r of a lane: feature 16 half + r
-                    const long long feat = feat0 + wfeat + n * 32 + half * 16 + q * kE, left = kWhole ? kE : nfeat - feat;
-                    if (left <= 0) continue;
-                    float v[kE];
-#pragma unroll
-                    for (int j = 0; j < kE; j++) v[j] = acc[n][m][kE * q + j];
-                    if (P == kForward) {
-                        float s[kE];
-                        if (a.b) {
-                            const auto b = load_n<T, kE>((const T*)a.b + feat, left);
-#pragma unroll
-                            for (int j = 0; j < kE; j++) v[j] += to_f(b.e[j]);
-                        }
-#pragma unroll
-                        for (int j = 0; j < kE; j++) v[j] = activate<sizeof(T) == 4>(v[j], a.act, s[j]);
-                        if (a.slope) store_n<Slope, kE>((Slope*)a.slope + row * a.out + feat, left, s);
-                        if (a.res) {
-                            const auto b = load_n<T, kE>((const T*)a.res + row * a.res_ld + feat, left);
-#pragma unroll
-                            for (int j = 0; j < kE; j++) v[j] += to_f(b.e[j]);
-                        }
-                        store_n<T, kE>((T*)a.y + row * a.y_ld + feat, left, v);
-                    } else if (P == kInput) {
-                        store_n<T, kE>((T*)a.dx + row * a.dx_ld + feat, left, v);
-                    } else {
-                        store_n<float, kE>(a.work + unit.part * a.out * a.in + row * a.in + feat, left, v);
-                    }
-                }
-        }
-    };
-    if (feat0 + BN <= nfeat) epilogue(std::true_type{}); else epilogue(std::false_type{});
+    write_results<T, P, TM, TN>(a, acc, row0 + wrow, nrows, feat0 + wfeat, nfeat, feat0 + BN <= nfeat, unit.part);
     if constexpr (P == kWeight) {
         if (want_db) {  // threads of one row group hold the sums of eight reduction pieces: joined in order through LDS
             float* join = (float*)lds;
@@ -384,16 +441,203 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_kernel(LinearArgs a, int 
     }
 }
 
+// ---- the same three products with operands whose rows are whole, aligned 16-byte pieces (dz already formed): the tiles go
+// from memory to LDS without passing through registers, one tile ahead of the matrix cores. A [reduction][row] operand
+// keeps its order in LDS and is turned by the transposing LDS reads (16-bit types; f32 fragments are single values). ----
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// Natural tile of ROWS features: kE-element pieces, kP a row; the piece index is XORed by the reduction step so that the
+// four (16-bit) or two (f32) steps one LDS access touches lie in different banks.
+template <class T, int ROWS> struct NaturalSwz {
+    static constexpr int kP = ROWS / Elem<T>::kE;
+    static __device__ __forceinline__ int of(int m) { return sizeof(T) == 2 ? (kP >= 16 ? 4 * (m & 3) : 4 * ((m >> 1) & 1)) : kP >= 16 ? 8 * ((m >> 2) & 1) : 0; }
+};
+
+template <class T, int ROWS, int WAVES, bool NATURAL, bool FEATURES>
+struct StreamTile {
+    static constexpr int kE = Elem<T>::kE, kP = ROWS / kE, kN = ROWS * kPieces / 64 / WAVES;
+    static_assert(ROWS * kPieces % (64 * WAVES) == 0, "a whole number of loads for each wave");
+    const T* base[kN];
+    long long step;  // elements from one reduction step to the next
+    __device__ __forceinline__ static int slot(int i) { return ((threadIdx.x >> 6) + i * WAVES) * 64 + (threadIdx.x & 63); }
+    __device__ __forceinline__ static int offset(int i) {  // of the lane's piece, in reduction steps
+        const int s = slot(i);
+        return NATURAL ? s / kP : ((s & 7) ^ swz(s >> 3)) * kE;
+    }
+    __device__ __forceinline__ void init(const T* p, long long ld, long long row0, long long rows) {
+        step = NATURAL ? ld : 1;
+#pragma unroll
+        for (int i = 0; i < kN; i++) {
+            const int s = slot(i);
+            if (NATURAL) {
+                const int m = s / kP;
+                long long f = row0 + ((s % kP) ^ NaturalSwz<T, ROWS>::of(m)) * kE;
+                f = f < rows ? f : rows - kE;  // past the end: any piece of the row, its results are not stored
+                base[i] = p + m * ld + f;
+            } else {
+                long long r = row0 + (FEATURES ? feature_of(s >> 3) : s >> 3);
+                r = r < rows ? r : rows - 1;
+                base[i] = p + r * ld + offset(i);
+            }
+        }
+    }
+    // A whole tile from reduction step k on, straight into LDS: a wave's 64 lanes fill 1 KiB in order.
+    __device__ __forceinline__ void stage(u32x4* lds, long long k) const {
+#pragma unroll
+        for (int i = 0; i < kN; i++)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(base[i] + k * step),
+                                             (__attribute__((address_space(3))) void*)(lds + ((threadIdx.x >> 6) + i * WAVES) * 64), 16, 0, 0);
+    }
+    // The last, partial tile: zeros past the end of the reduction.
+    __device__ __forceinline__ void stage_end(u32x4* lds, long long k, long long kend) const {
+#pragma unroll
+        for (int i = 0; i < kN; i++) {
+            u32x4 v = {0, 0, 0, 0};
+            if (k + offset(i) < kend) v = *(const u32x4*)(base[i] + k * step);
+            lds[slot(i)] = v;
+        }
+    }
+    // The lane's fragment of rows block ... block + 31 at step s (32 bytes of reduction).
+    __device__ __forceinline__ static u32x4 fragment(const u32x4* lds, int block, int s) {
+        const int lane = threadIdx.x & 63, half = lane >> 5, l32 = lane & 31;
+        if constexpr (!NATURAL) {
+            const int r = block + l32;
+            return lds[r * kPieces + ((2 * s + half) ^ swz(r))];
+        } else if constexpr (sizeof(T) == 2) {
+            // sixteen lanes turn a block of four steps x 16 features: lane j points at step j / 4, features 4 (j % 4) ...
+            const int i = (lane & 16) + 4 * (lane & 3), f = block + (FEATURES ? feature_of(i) : i), m0 = (lane & 15) >> 2;
+            union { u32x4 u; s16x4 h[2]; } v;
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const int m = 16 * s + 8 * half + 4 * t + m0;
+                const char* at = (const char*)(lds + m * kP + ((f / kE) ^ NaturalSwz<T, ROWS>::of(m))) + f % kE * 2;
+                v.h[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+            }
+            return v.u;
+        } else {
+            const int f = block + (FEATURES ? feature_of(l32) : l32);
+            u32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int m = 8 * s + 4 * half + e;
+                v[e] = ((const uint32_t*)(lds + m * kP + ((f / kE) ^ NaturalSwz<T, ROWS>::of(m))))[f % kE];
+            }
+            return v;
+        }
+    }
+};
+
+template <class T, Product P, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64, 2) void linear_stream_kernel(LinearArgs a, int tiles_n, long long tiles, int parts, long long red_part) {
+    constexpr int kE = Elem<T>::kE, kK = kPieces * kE, TM = BM / WM / 32, TN = BN / WN / 32;
+    __shared__ u32x4 lds[2][(BM + BN) * kPieces];
+    const Unit unit = unit_of(tiles, tiles_n, tiles * parts);
+    if (unit.none) return;
+    long long nrows, nfeat, red0 = 0, red1;
+    const long long row0 = unit.tm * BM, feat0 = (long long)unit.tn * BN;
+    StreamTile<T, BM, WM * WN, P == kWeight, false> rt;
+    StreamTile<T, BN, WM * WN, P != kForward, true> ft;
+    if (P == kForward) {
+        nrows = a.rows; nfeat = a.out; red1 = a.in;
+        rt.init((const T*)a.x, a.x_ld, row0, nrows);
+        ft.init((const T*)a.w, a.w_ld, feat0, nfeat);
+    } else if (P == kInput) {
+        nrows = a.rows; nfeat = a.in; red1 = a.out;
+        rt.init((const T*)a.dy, a.dy_ld, row0, nrows);
+        ft.init((const T*)a.w, a.w_ld, feat0, nfeat);
+    } else {
+        nrows = a.out; nfeat = a.in;
+        red0 = unit.part * red_part;
+        red1 = red0 + red_part < a.rows ? red0 + red_part : a.rows;
+        rt.init((const T*)a.dy, a.dy_ld, row0, nrows);
+        ft.init((const T*)a.x, a.x_ld, feat0, nfeat);
+    }
+    auto stage = [&](int to, long long k) {
+        if (k + kK <= red1) {
+            rt.stage(lds[to], k);
+            ft.stage(lds[to] + BM * kPieces, k);
+        } else {
+            rt.stage_end(lds[to], k, red1);
+            ft.stage_end(lds[to] + BM * kPieces, k, red1);
+        }
+    };
+    f32x16 acc[TN][TM] = {};
+    const int wave = threadIdx.x >> 6, wrow = (wave / WN) * TM * 32, wfeat = (wave % WN) * TN * 32;
+    int buf = 0;
+    if (red0 < red1) stage(0, red0);
+    for (long long k = red0; k < red1; k += kK, buf ^= 1) {
+        __syncthreads();  // this tile has landed, and everyone has left the other one
+        if (k + kK < red1) stage(buf ^ 1, k + kK);
+        const u32x4* lr = lds[buf];
+        const u32x4* lf = lds[buf] + BM * kPieces;
+#pragma unroll
+        for (int s = 0; s < kPieces / 2; s++) {
+            u32x4 fr[TM], ff[TN];
+#pragma unroll
+            for (int i = 0; i < TM; i++) fr[i] = rt.fragment(lr, wrow + i * 32, s);
+#pragma unroll
+            for (int i = 0; i < TN; i++) ff[i] = ft.fragment(lf, wfeat + i * 32, s);
+#pragma unroll
+            for (int n = 0; n < TN; n++)
+#pragma unroll
+                for (int m = 0; m < TM; m++) mfma(acc[n][m], ff[n], fr[m], T{});
+        }
+    }
+    write_results<T, P, TM, TN>(a, acc, row0 + wrow, nrows, feat0 + wfeat, nfeat, feat0 + BN <= nfeat, unit.part);
+}
+
+// dz = dy * slope, rounded once to T, into a dense [rows][out] buffer (or nowhere: dz is dy), and the bias gradient's partial
+// sums of the 32-bit values: thread (c, g) of a workgroup owns piece c of a strip of kStrip pieces and every kGroups-th of the
+// workgroup's rows.
+template <class T>
+__global__ __launch_bounds__(256) void linear_dz_kernel(LinearArgs a, T* dz, float* partial, long long rows_part) {
+    using Slope = typename Elem<T>::Slope;
+    constexpr int kE = Elem<T>::kE, kStrip = 32, kGroups = 8;
+    __shared__ float join[kGroups][kStrip * kE];
+    const int c = threadIdx.x % kStrip, g = threadIdx.x / kStrip;
+    const long long col = ((long long)blockIdx.y * kStrip + c) * kE, left = a.out - col;
+    const long long row0 = blockIdx.x * rows_part, row1 = row0 + rows_part < a.rows ? row0 + rows_part : a.rows;
+    float sum[kE] = {};
+    if (left > 0)
+#pragma unroll 4
+        for (long long r = row0 + g; r < row1; r += kGroups) {
+            const auto v = load_n<T, kE>((const T*)a.dy + r * a.dy_ld + col, kE);
+            float f[kE];
+#pragma unroll
+            for (int e = 0; e < kE; e++) f[e] = to_f(v.e[e]);
+            if (a.slope) {
+                const auto q = load_n<Slope, kE>((const Slope*)a.slope + r * a.out + col, kE);
+#pragma unroll
+                for (int e = 0; e < kE; e++) f[e] *= to_f(q.e[e]);
+            }
+            if (dz) store_n<T, kE>(dz + r * a.out + col, kE, f);
+#pragma unroll
+            for (int e = 0; e < kE; e++) sum[e] += f[e];
+        }
+    if (!partial) return;
+#pragma unroll
+    for (int e = 0; e < kE; e++) join[g][c * kE + e] = sum[e];
+    __syncthreads();
+    const long long first = (long long)blockIdx.y * kStrip * kE;
+    for (int i = threadIdx.x; i < kStrip * kE && first + i < a.out; i += 256) {
+        float s = 0.f;
+#pragma unroll
+        for (int k = 0; k < kGroups; k++) s += join[k][i];
+        partial[(long long)blockIdx.x * a.out + first + i] = s;
+    }
+}
+
 // Joins the partial sums of the weight and bias gradients in a fixed order, 32 values a workgroup, eight threads a value:
 // every result is the same in every run.
 template <class T>
-__global__ __launch_bounds__(kJoinThreads) void linear_join_kernel(const float* work, T* dw, T* db, long long weights, int out, int parts) {
+__global__ __launch_bounds__(kJoinThreads) void linear_join_kernel(const float* work, const float* db_work, T* dw, T* db, long long weights, int out, int w_parts, int b_parts) {
     __shared__ float join[8][32];
     const int c = threadIdx.x & 31, slice = threadIdx.x >> 5;
     const long long i = (long long)blockIdx.x * 32 + c, nw = dw ? weights : 0, all = nw + (db ? out : 0);
     const bool is_w = i < nw;
     const long long at = is_w ? i : i - nw, step = is_w ? weights : out;
-    const float* p = is_w ? work + at : work + parts * weights + at;
+    const float* p = (is_w ? work : db_work) + at;
+    const int parts = is_w ? w_parts : b_parts;
     float s = 0.f;
     if (i < all)
 #pragma unroll 4
@@ -451,19 +695,75 @@ int weight_grad(const LinearArgs& a, const Split& sp, hipStream_t s) {
     return launch<T, kWeight, 128, 128, 2, 2>(a, a.out, a.in, sp.parts, part, s);
 }
 
+template <class T, Product P, int BM, int BN, int WM, int WN>
+int stream(const LinearArgs& a, long long nrows, long long nfeat, int parts, long long red_part, hipStream_t s) {
+    const int tiles_n = (int)((nfeat + BN - 1) / BN);
+    const long long tiles = (nrows + BM - 1) / BM * tiles_n, units = tiles * parts;
+    linear_stream_kernel<T, P, BM, BN, WM, WN><<<(unsigned)((units + 7) / 8 * 8), WM * WN * 64, 0, s>>>(a, tiles_n, tiles, parts, red_part);
+    return (int)hipGetLastError();
+}
+
+template <class T, Product P>
+int stream_product(const LinearArgs& a, long long feats, hipStream_t s) {
+    if (feats <= 64) return stream<T, P, 128, 64, 4, 1>(a, a.rows, feats, 1, 0, s);
+    return stream<T, P, 128, 128, 2, 2>(a, a.rows, feats, 1, 0, s);
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+constexpr int kDzParts = 512;
+
+// Whether the backward pass forms dz in a pass of its own and streams both products.
+template <class T>
+bool streams_backward(const LinearArgs& a) {
+    constexpr int kE = Elem<T>::kE;
+    return a.in % kE == 0 && a.out % kE == 0 && a.w_ld % kE == 0 && a.dy_ld % kE == 0 && a.x_ld % kE == 0 && aligned16(a.w) && aligned16(a.dy) && aligned16(a.x) && aligned16(a.slope) &&
+           a.in > 64 && a.out > 64 && !few(a.rows, a.in);
+}
+
+template <class T>
+int backward_stream(LinearArgs a, hipStream_t s) {
+    constexpr int kE = Elem<T>::kE, kK = kPieces * kE;
+    const Split sp = split_of(a.rows, a.in, a.out);
+    const long long weights = (long long)a.out * a.in;
+    float* db_work = a.work + sp.parts * weights;
+    T* dz = (T*)(db_work + ((long long)kDzParts * a.out + 3) / 4 * 4);
+    const long long rows_part = (a.rows + kDzParts - 1) / kDzParts;
+    const int dz_parts = (int)((a.rows + rows_part - 1) / rows_part);
+    int rc = 0;
+    if (a.slope || a.db) {
+        linear_dz_kernel<T><<<dim3(dz_parts, (a.out + 32 * kE - 1) / (32 * kE)), 256, 0, s>>>(a, a.slope && (a.dx || a.dw) ? dz : nullptr, a.db ? db_work : nullptr, rows_part);
+        if ((rc = (int)hipGetLastError())) return rc;
+    }
+    if (a.slope) { a.dy = dz; a.dy_ld = a.out; }
+    if (a.dx && (rc = stream_product<T, kInput>(a, a.in, s))) return rc;
+    if (a.dw) {
+        const long long part = ((a.rows + sp.parts - 1) / sp.parts + kK - 1) / kK * kK;
+        if ((rc = stream<T, kWeight, 128, 128, 2, 2>(a, a.out, a.in, sp.parts, part, s))) return rc;
+    }
+    if (!a.dw && !a.db) return 0;
+    const long long all = (a.dw ? weights : 0) + (a.db ? a.out : 0);
+    linear_join_kernel<T><<<(unsigned)((all + 31) / 32), kJoinThreads, 0, s>>>(a.work, db_work, (T*)a.dw, (T*)a.db, weights, a.out, sp.parts, dz_parts);
+    return (int)hipGetLastError();
+}
+
+template <class T>
+int forward_any(const LinearArgs& a, hipStream_t s) {
+    constexpr int kE = Elem<T>::kE;
+    if (a.in % kE == 0 && a.x_ld % kE == 0 && a.w_ld % kE == 0 && aligned16(a.x) && aligned16(a.w) && a.out > 32 && !few(a.rows, a.out)) return stream_product<T, kForward>(a, a.out, s);
+    return product<T, kForward>(a, a.out, s);
+}
+
 template <class T>
 int backward_any(const LinearArgs& a, hipStream_t s) {
+    if (streams_backward<T>(a)) return backward_stream<T>(a, s);
     int rc = 0;
-    if (a.dx && a.rows) {
-        rc = product<T, kInput>(a, a.in, s);
-        if (rc) return rc;
-    }
+    if (a.dx && a.rows && (rc = product<T, kInput>(a, a.in, s))) return rc;
     if (a.dw || a.db) {
         const Split sp = split_of(a.rows, a.in, a.out);
-        rc = weight_grad<T>(a, sp, s);
-        if (rc) return rc;
+        if ((rc = weight_grad<T>(a, sp, s))) return rc;
         const long long weights = (long long)a.out * a.in, all = (a.dw ? weights : 0) + (a.db ? a.out : 0);
-        linear_join_kernel<T><<<(unsigned)((all + 31) / 32), kJoinThreads, 0, s>>>(a.work, (T*)a.dw, (T*)a.db, weights, a.out, sp.parts);
+        linear_join_kernel<T><<<(unsigned)((all + 31) / 32), kJoinThreads, 0, s>>>(a.work, a.work + sp.parts * weights, (T*)a.dw, (T*)a.db, weights, a.out, sp.parts, sp.parts);
         rc = (int)hipGetLastError();
     }
     return rc;
@@ -473,13 +773,16 @@ int backward_any(const LinearArgs& a, hipStream_t s) {
 
 int linear_forward_launch(int dtype, const LinearArgs& a, hipStream_t s) {
     if (!a.rows) return 0;
-    return dtype == DRONE_F32 ? product<float, kForward>(a, a.out, s) : dtype == DRONE_BF16 ? product<__bf16, kForward>(a, a.out, s) : product<_Float16, kForward>(a, a.out, s);
+    return dtype == DRONE_F32 ? forward_any<float>(a, s) : dtype == DRONE_BF16 ? forward_any<__bf16>(a, s) : forward_any<_Float16>(a, s);
 }
 int linear_backward_launch(int dtype, const LinearArgs& a, hipStream_t s) {
     return dtype == DRONE_F32 ? backward_any<float>(a, s) : dtype == DRONE_BF16 ? backward_any<__bf16>(a, s) : backward_any<_Float16>(a, s);
 }
-size_t linear_work_bytes(int, long long rows, int in, int out) {
-    return (size_t)split_of(rows, in, out).parts * ((size_t)in * out + out) * sizeof(float);
+size_t linear_work_bytes(int dtype, long long rows, int in, int out) {
+    // (whether the backward pass streams depends on alignment too: room for either)
+    const Split sp = split_of(rows, in, out);
+    const size_t dz = in > 64 && out > 64 && !few(rows, in) ? ((size_t)kDzParts * out + 4) * sizeof(float) + (size_t)rows * out * (dtype == DRONE_F32 ? 4 : 2) : 0;
+    return (size_t)sp.parts * ((size_t)in * out + out) * sizeof(float) + dz;
 }
 
 }  // namespace drone
