@@ -6,7 +6,6 @@ has no binding source (``/root/reference/.gitmodules:1-3`` names an empty
 submodule).
 """
 import ctypes as C
-import struct
 
 OBS_DIM = 20
 OBS_DIM_MAX = 24
@@ -120,14 +119,6 @@ class DroneAdamW(C.Structure):
     ]
 
 
-# The same blocks as struct formats: one pack() builds a call's bytes (the calls take any pointer), a tenth of the time of
-# filling a ctypes structure field by field.
-LINEAR_CALL = struct.Struct("@Iiii3q10P6qPQ")
-NORM_CALL = struct.Struct("@Iiii2q14P3q2fPQ")
-ADAMW_TENSOR = struct.Struct("@5Pq")
-ADAMW_CALL = struct.Struct("@Iiii3P6dPQ")
-
-
 # numpy structured dtype with the same layout as DroneStateRow (33 words).
 def state_row_dtype():
     import numpy as np
@@ -190,14 +181,14 @@ SYMBOLS = {
     "drone_device_malloc": (_P, [C.c_int, C.c_size_t]),
     "drone_device_free": (None, [C.c_int, _P]),
     "drone_vec_copy_to_host": (C.c_int, [_P, _P, _P, C.c_size_t]),
-    "drone_linear_forward": (C.c_int, [_P, _P]),
-    "drone_linear_backward": (C.c_int, [_P, _P]),
-    "drone_linear_workspace": (C.c_uint64, [_P]),
-    "drone_norm_forward": (C.c_int, [_P, _P]),
-    "drone_norm_backward": (C.c_int, [_P, _P]),
-    "drone_norm_workspace": (C.c_uint64, [_P]),
-    "drone_adamw_step": (C.c_int, [_P, _P]),
-    "drone_adamw_workspace": (C.c_uint64, [_P]),
+    "drone_linear_forward": (C.c_int, [C.POINTER(DroneLinear), _P]),
+    "drone_linear_backward": (C.c_int, [C.POINTER(DroneLinear), _P]),
+    "drone_linear_workspace": (C.c_uint64, [C.POINTER(DroneLinear)]),
+    "drone_norm_forward": (C.c_int, [C.POINTER(DroneNorm), _P]),
+    "drone_norm_backward": (C.c_int, [C.POINTER(DroneNorm), _P]),
+    "drone_norm_workspace": (C.c_uint64, [C.POINTER(DroneNorm)]),
+    "drone_adamw_step": (C.c_int, [C.POINTER(DroneAdamW), _P]),
+    "drone_adamw_workspace": (C.c_uint64, [C.POINTER(DroneAdamW)]),
     "drone_vec_timer_start": (C.c_int, [_P]),
     "drone_vec_timer_stop": (C.c_int, [_P, C.POINTER(C.c_float)]),
     "drone_last_error": (C.c_char_p, []),

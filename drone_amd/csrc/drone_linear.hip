@@ -453,16 +453,20 @@ template <class T, int ROWS> struct NaturalSwz {
     static __device__ __forceinline__ int of(int m) { return sizeof(T) == 2 ? (kP >= 16 ? 4 * (m & 3) : 4 * ((m >> 1) & 1)) : kP >= 16 ? 8 * ((m >> 2) & 1) : 0; }
 };
 
-template <class T, int ROWS, int WAVES, bool NATURAL, bool FEATURES>
+// PIECES 16-byte pieces of the reduction a row. Contiguous tiles: piece p of row r at p ^ piece_swz(r), so that the sixteen
+// rows one LDS access takes lie in different banks.
+template <int PIECES> __device__ __forceinline__ int piece_swz(int r) { return PIECES == 8 ? swz(r) : (r >> 2) & 3; }
+
+template <class T, int ROWS, int PIECES, int WAVES, bool NATURAL, bool FEATURES>
 struct StreamTile {
-    static constexpr int kE = Elem<T>::kE, kP = ROWS / kE, kN = ROWS * kPieces / 64 / WAVES;
-    static_assert(ROWS * kPieces % (64 * WAVES) == 0, "a whole number of loads for each wave");
+    static constexpr int kE = Elem<T>::kE, kP = ROWS / kE, kN = ROWS * PIECES / 64 / WAVES;
+    static_assert(ROWS * PIECES % (64 * WAVES) == 0, "a whole number of loads for each wave");
     const T* base[kN];
     long long step;  // elements from one reduction step to the next
     __device__ __forceinline__ static int slot(int i) { return ((threadIdx.x >> 6) + i * WAVES) * 64 + (threadIdx.x & 63); }
     __device__ __forceinline__ static int offset(int i) {  // of the lane's piece, in reduction steps
         const int s = slot(i);
-        return NATURAL ? s / kP : ((s & 7) ^ swz(s >> 3)) * kE;
+        return NATURAL ? s / kP : ((s % PIECES) ^ piece_swz<PIECES>(s / PIECES)) * kE;
     }
     __device__ __forceinline__ void init(const T* p, long long ld, long long row0, long long rows) {
         step = NATURAL ? ld : 1;
@@ -475,7 +479,7 @@ struct StreamTile {
                 f = f < rows ? f : rows - kE;  // past the end: any piece of the row, its results are not stored
                 base[i] = p + m * ld + f;
             } else {
-                long long r = row0 + (FEATURES ? feature_of(s >> 3) : s >> 3);
+                long long r = row0 + (FEATURES ? feature_of(s / PIECES) : s / PIECES);
                 r = r < rows ? r : rows - 1;
                 base[i] = p + r * ld + offset(i);
             }
@@ -502,7 +506,7 @@ struct StreamTile {
         const int lane = threadIdx.x & 63, half = lane >> 5, l32 = lane & 31;
         if constexpr (!NATURAL) {
             const int r = block + l32;
-            return lds[r * kPieces + ((2 * s + half) ^ swz(r))];
+            return lds[r * PIECES + ((2 * s + half) ^ piece_swz<PIECES>(r))];
         } else if constexpr (sizeof(T) == 2) {
             // sixteen lanes turn a block of four steps x 16 features: lane j points at step j / 4, features 4 (j % 4) ...
             const int i = (lane & 16) + 4 * (lane & 3), f = block + (FEATURES ? feature_of(i) : i), m0 = (lane & 15) >> 2;
@@ -527,16 +531,26 @@ struct StreamTile {
     }
 };
 
-template <class T, Product P, int BM, int BN, int WM, int WN>
+// Waits until at most LEFT of the wave's loads are under way (its LDS accesses all done), then for the workgroup.
+template <int LEFT>
+__device__ __forceinline__ void landed() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LEFT) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+template <class T, Product P, int BM, int BN, int WM, int WN, int PIECES, int STAGES>
 __global__ __launch_bounds__(WM * WN * 64, 2) void linear_stream_kernel(LinearArgs a, int tiles_n, long long tiles, int parts, long long red_part) {
-    constexpr int kE = Elem<T>::kE, kK = kPieces * kE, TM = BM / WM / 32, TN = BN / WN / 32;
-    __shared__ u32x4 lds[2][(BM + BN) * kPieces];
+    constexpr int kE = Elem<T>::kE, kK = PIECES * kE, TM = BM / WM / 32, TN = BN / WN / 32;
+    __shared__ u32x4 lds[STAGES][(BM + BN) * PIECES];
     const Unit unit = unit_of(tiles, tiles_n, tiles * parts);
     if (unit.none) return;
     long long nrows, nfeat, red0 = 0, red1;
     const long long row0 = unit.tm * BM, feat0 = (long long)unit.tn * BN;
-    StreamTile<T, BM, WM * WN, P == kWeight, false> rt;
-    StreamTile<T, BN, WM * WN, P != kForward, true> ft;
+    using RowTile = StreamTile<T, BM, PIECES, WM * WN, P == kWeight, false>;
+    using FeatTile = StreamTile<T, BN, PIECES, WM * WN, P != kForward, true>;
+    RowTile rt;
+    FeatTile ft;
     if (P == kForward) {
         nrows = a.rows; nfeat = a.out; red1 = a.in;
         rt.init((const T*)a.x, a.x_ld, row0, nrows);
@@ -555,33 +569,38 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void linear_stream_kernel(LinearAr
     auto stage = [&](int to, long long k) {
         if (k + kK <= red1) {
             rt.stage(lds[to], k);
-            ft.stage(lds[to] + BM * kPieces, k);
-        } else {
+            ft.stage(lds[to] + BM * PIECES, k);
+        } else if (k < red1) {
             rt.stage_end(lds[to], k, red1);
-            ft.stage_end(lds[to] + BM * kPieces, k, red1);
+            ft.stage_end(lds[to] + BM * PIECES, k, red1);
         }
     };
     f32x16 acc[TN][TM] = {};
     const int wave = threadIdx.x >> 6, wrow = (wave / WN) * TM * 32, wfeat = (wave % WN) * TN * 32;
-    int buf = 0;
-    if (red0 < red1) stage(0, red0);
-    for (long long k = red0; k < red1; k += kK, buf ^= 1) {
-        __syncthreads();  // this tile has landed, and everyone has left the other one
-        if (k + kK < red1) stage(buf ^ 1, k + kK);
-        const u32x4* lr = lds[buf];
-        const u32x4* lf = lds[buf] + BM * kPieces;
+    // STAGES - 1 tiles under way. Tile i's loads are the oldest when its turn comes: the wait leaves the later tiles' out.
 #pragma unroll
-        for (int s = 0; s < kPieces / 2; s++) {
+    for (int i = 0; i < STAGES - 1; i++) stage(i, red0 + (long long)i * kK);
+    int buf = 0;
+    for (long long k = red0; k < red1; k += kK) {
+        if (k + (long long)(STAGES - 1) * kK <= red1) landed<(STAGES - 2) * (RowTile::kN + FeatTile::kN)>();
+        else landed<0>();  // the last tiles: fewer, or one that went through registers, are behind this one
+        const int next = buf == 0 ? STAGES - 1 : buf - 1;  // whose tile everyone has left at this barrier
+        stage(next, k + (long long)(STAGES - 1) * kK);
+        const u32x4* lr = lds[buf];
+        const u32x4* lf = lds[buf] + BM * PIECES;
+#pragma unroll
+        for (int s = 0; s < PIECES / 2; s++) {
             u32x4 fr[TM], ff[TN];
 #pragma unroll
-            for (int i = 0; i < TM; i++) fr[i] = rt.fragment(lr, wrow + i * 32, s);
+            for (int i = 0; i < TM; i++) fr[i] = RowTile::fragment(lr, wrow + i * 32, s);
 #pragma unroll
-            for (int i = 0; i < TN; i++) ff[i] = ft.fragment(lf, wfeat + i * 32, s);
+            for (int i = 0; i < TN; i++) ff[i] = FeatTile::fragment(lf, wfeat + i * 32, s);
 #pragma unroll
             for (int n = 0; n < TN; n++)
 #pragma unroll
                 for (int m = 0; m < TM; m++) mfma(acc[n][m], ff[n], fr[m], T{});
         }
+        buf = buf == STAGES - 1 ? 0 : buf + 1;
     }
     write_results<T, P, TM, TN>(a, acc, row0 + wrow, nrows, feat0 + wfeat, nfeat, feat0 + BN <= nfeat, unit.part);
 }
@@ -695,18 +714,18 @@ int weight_grad(const LinearArgs& a, const Split& sp, hipStream_t s) {
     return launch<T, kWeight, 128, 128, 2, 2>(a, a.out, a.in, sp.parts, part, s);
 }
 
-template <class T, Product P, int BM, int BN, int WM, int WN>
+template <class T, Product P, int BM, int BN, int WM, int WN, int PIECES, int STAGES>
 int stream(const LinearArgs& a, long long nrows, long long nfeat, int parts, long long red_part, hipStream_t s) {
     const int tiles_n = (int)((nfeat + BN - 1) / BN);
     const long long tiles = (nrows + BM - 1) / BM * tiles_n, units = tiles * parts;
-    linear_stream_kernel<T, P, BM, BN, WM, WN><<<(unsigned)((units + 7) / 8 * 8), WM * WN * 64, 0, s>>>(a, tiles_n, tiles, parts, red_part);
+    linear_stream_kernel<T, P, BM, BN, WM, WN, PIECES, STAGES><<<(unsigned)((units + 7) / 8 * 8), WM * WN * 64, 0, s>>>(a, tiles_n, tiles, parts, red_part);
     return (int)hipGetLastError();
 }
 
 template <class T, Product P>
 int stream_product(const LinearArgs& a, long long feats, hipStream_t s) {
-    if (feats <= 64) return stream<T, P, 128, 64, 4, 1>(a, a.rows, feats, 1, 0, s);
-    return stream<T, P, 128, 128, 2, 2>(a, a.rows, feats, 1, 0, s);
+    if (feats <= 64) return stream<T, P, 128, 64, 4, 1, 8, 2>(a, a.rows, feats, 1, 0, s);
+    return stream<T, P, 128, 128, 2, 2, 8, 2>(a, a.rows, feats, 1, 0, s);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -739,7 +758,7 @@ int backward_stream(LinearArgs a, hipStream_t s) {
     if (a.dx && (rc = stream_product<T, kInput>(a, a.in, s))) return rc;
     if (a.dw) {
         const long long part = ((a.rows + sp.parts - 1) / sp.parts + kK - 1) / kK * kK;
-        if ((rc = stream<T, kWeight, 128, 128, 2, 2>(a, a.out, a.in, sp.parts, part, s))) return rc;
+        if ((rc = stream<T, kWeight, 128, 128, 2, 2, 8, 2>(a, a.out, a.in, sp.parts, part, s))) return rc;
     }
     if (!a.dw && !a.db) return 0;
     const long long all = (a.dw ? weights : 0) + (a.db ? a.out : 0);

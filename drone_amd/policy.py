@@ -18,117 +18,23 @@ import torch
 
 from . import abi, binding
 
-_DTYPES = {torch.float32: abi.F32, torch.bfloat16: abi.BF16, torch.float16: abi.F16}
+_native_module = None
 
 
-def _fail(what):
-    raise RuntimeError(f"libdrone_hip: {binding.last_error() or what}")
-
-
-def _call(name, blob, device):
-    """One C-ABI call on torch's current stream of the device."""
-    if binding.functions()[name](blob, torch.cuda.current_stream(device).cuda_stream):
-        _fail(name)
-
-
-def _workspace(name, blob, device):
-    return torch.empty(binding.functions()[name](blob), dtype=torch.uint8, device=device)
-
-
-def _ptr(t):
-    return 0 if t is None else t.data_ptr()
-
-
-def _check(name, t, shape, like):
-    """A tensor argument: its shape, and the type and device of ``like``."""
-    if t is None:
-        return
-    if tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if t.dtype != like.dtype:
-        raise TypeError(f"{name} is {t.dtype}, x is {like.dtype}")
-    if t.device != like.device:
-        raise ValueError(f"{name} is on {t.device}, x on {like.device}")
-
-
-def _check_x(x, name="x"):
-    if x.dtype not in _DTYPES:
-        raise TypeError(f"{name} is {x.dtype}: float32, bfloat16 or float16")
-    if x.device.type != "cuda":
-        raise ValueError(f"{name} is on {x.device}: the policy operators run on a GPU only")
-
-
-def _rows(t):
-    """A tensor [..., n] as [rows][n] with contiguous rows and a leading dimension of at least n: a view where there is
-    one, else a copy. Overlapping rows (an expanded tensor) are copied."""
-    if t is None:
-        return None
-    n = t.shape[-1]
-    if t.dim() != 2:
-        t = t.reshape(-1, n)
-    if (n > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < n):
-        t = t.contiguous()
-    return t
-
-
-def _ld(t):
-    return 0 if t is None else max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
-
-
-def _slope_type(dtype):
-    return torch.float16 if dtype == torch.bfloat16 else torch.float32
-
-
-_LINEAR_SIZE, _NORM_SIZE, _ADAMW_SIZE = abi.LINEAR_CALL.size, abi.NORM_CALL.size, abi.ADAMW_CALL.size
-
-
-def _linear_forward(x, weight, bias, residual, activation, slope, y=None):
-    n, k = weight.shape
-    rows = x.shape[0]
-    if y is None:
-        y = x.new_empty((rows, n))
-    _call("drone_linear_forward", abi.LINEAR_CALL.pack(
-        _LINEAR_SIZE, x.get_device(), _DTYPES[x.dtype], activation, rows, k, n,
-        x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(residual), 0, y.data_ptr(), _ptr(slope), 0, 0, 0,
-        _ld(x), _ld(weight), _ld(residual), 0, _ld(y), 0, 0, 0), x.device)
-    return y
-
-
-class _LinearFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, activation):
-        slope = torch.empty((x.shape[0], weight.shape[0]), dtype=_slope_type(x.dtype), device=x.device) if activation else None
-        y = _linear_forward(x, weight, bias, residual, activation, slope)
-        ctx.activation = activation
-        ctx.save_for_backward(x, weight, slope)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, weight, slope = ctx.saved_tensors
-        want_x, want_w, want_b, want_r = ctx.needs_input_grad[:4]
-        dx = dw = db = work = None
-        if want_x or want_w or want_b:
-            d = _rows(dy)
-            n, k = weight.shape
-            if want_x:
-                dx = x.new_empty((x.shape[0], k))
-            if want_w:
-                dw = x.new_empty((n, k))
-            if want_b:
-                db = x.new_empty(n)
-
-            def blob(work):
-                return abi.LINEAR_CALL.pack(
-                    _LINEAR_SIZE, x.get_device(), _DTYPES[x.dtype], ctx.activation, x.shape[0], k, n,
-                    x.data_ptr(), weight.data_ptr(), 0, 0, d.data_ptr(), 0, _ptr(slope), _ptr(dx), _ptr(dw), _ptr(db),
-                    _ld(x), _ld(weight), 0, _ld(d), 0, k, _ptr(work), 0 if work is None else work.numel())
-
-            if want_w or want_b:
-                work = _workspace("drone_linear_workspace", blob(None), x.device)
-            _call("drone_linear_backward", blob(work), x.device)
-        return dx, dw, db, dy if want_r else None, None
+def _native():
+    """The compiled module over the C-ABI (bindings/policy_torch.cpp), given the loaded library's entry points on first use."""
+    global _native_module
+    if _native_module is None:
+        lib = binding.load()
+        try:
+            from . import policy_torch
+        except ImportError as e:
+            raise RuntimeError("drone_amd/policy_torch is missing or does not load: build it first "
+                               f"(python -c 'import __graft_entry__ as g; g.build()' or make -C bindings): {e}") from e
+        names = [n for n in abi.SYMBOLS if n.startswith(("drone_linear", "drone_norm", "drone_adamw"))] + ["drone_last_error"]
+        policy_torch.bind({n: C.cast(getattr(lib, n), C.c_void_p).value for n in names})
+        _native_module = policy_torch
+    return _native_module
 
 
 def linear(x, weight, bias=None, activation="none", residual=None, out=None):
@@ -137,73 +43,8 @@ def linear(x, weight, bias=None, activation="none", residual=None, out=None):
     x ``[..., in]``, weight ``[out, in]``, bias ``[out]``, residual ``[..., out]``, one type (float32, bfloat16, float16)
     and one GPU; activation: none, relu, tanh, silu, gelu (the erf form). Sums are 32-bit, the result is rounded once.
     ``out``: a tensor to write instead of a new one (the env's action buffer), ``[..., out]`` with contiguous rows; only
-    where nothing is differentiated. Rows may be a strided view; anything else is copied first."""
-    _check_x(x)
-    if activation not in abi.ACTIVATIONS:
-        raise ValueError(f"unknown activation {activation!r}; one of {', '.join(abi.ACTIVATIONS)}")
-    if weight.dim() != 2 or x.dim() < 1:
-        raise ValueError(f"weight must be [out, in] and x [..., in], got {tuple(weight.shape)} and {tuple(x.shape)}")
-    n, k = weight.shape
-    lead = x.shape[:-1]
-    if x.shape[-1] != k:
-        raise ValueError(f"x has {x.shape[-1]} features, the weight takes {k}")
-    _check("weight", weight, (n, k), x)
-    _check("bias", bias, (n,), x)
-    _check("residual", residual, (*lead, n), x)
-    _check("out", out, (*lead, n), x)
-    act = abi.ACTIVATIONS[activation]
-    learn = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual))
-    if out is not None:
-        if learn:
-            raise ValueError("out= cannot be differentiated: call under torch.no_grad()")
-        o = out if out.dim() == 2 else out.view(-1, n)
-        if (n > 1 and o.stride(1) != 1) or (o.shape[0] > 1 and o.stride(0) < n):
-            raise ValueError("out must have contiguous rows that do not overlap")
-    args = _rows(x), _rows(weight), None if bias is None else bias.contiguous(), _rows(residual), act
-    if learn:
-        return _LinearFunction.apply(*args).view(*lead, n)
-    if out is not None:
-        _linear_forward(*args, None, o)
-        return out
-    return _linear_forward(*args, None).view(*lead, n)
-
-
-def _norm_blob(x, block, gate, post, pre, scale, eps, dr=None, dh=None, r=None, h=None, grads=(None,) * 5, work=None):
-    kind = 0 if gate is None else gate.dim()
-    dx, dblock, dgate, dpost, dpre = grads
-    return abi.NORM_CALL.pack(
-        _NORM_SIZE, x.get_device(), _DTYPES[x.dtype], kind, x.shape[0], x.shape[1],
-        x.data_ptr(), _ptr(block), _ptr(gate), _ptr(post), _ptr(pre), _ptr(dr), _ptr(dh),
-        _ptr(r), _ptr(h), _ptr(dx), _ptr(dblock), _ptr(dgate), _ptr(dpost), _ptr(dpre),
-        _ld(x), _ld(block), _ld(gate) if kind == 2 else 0, scale, eps, _ptr(work), 0 if work is None else work.numel())
-
-
-def _norm_forward(x, block, gate, post, pre, scale, eps):
-    r, h = x.new_empty((x.shape[0], x.shape[1])), x.new_empty((x.shape[0], x.shape[1]))
-    _call("drone_norm_forward", _norm_blob(x, block, gate, post, pre, scale, eps, r=r, h=h), x.device)
-    return r, h
-
-
-class _NormFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, block, gate, post, pre, scale, eps):
-        ctx.set_materialize_grads(False)
-        ctx.numbers = scale, eps
-        ctx.save_for_backward(x, block, gate, post, pre)
-        return _norm_forward(x, block, gate, post, pre, scale, eps)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dr, dh):
-        x, block, gate, post, pre = ctx.saved_tensors
-        if dr is None and dh is None:
-            return (None,) * 7
-        dr, dh = (None if d is None else d.contiguous() for d in (dr, dh))
-        grads = [t.new_empty(t.shape) if want else None for t, want in zip((x, block, gate, post, pre), ctx.needs_input_grad)]
-        args = (x, block, gate, post, pre, *ctx.numbers, dr, dh, None, None, grads)
-        work = _workspace("drone_norm_workspace", _norm_blob(*args), x.device)
-        _call("drone_norm_backward", _norm_blob(*args, work), x.device)
-        return (*grads, None, None)
+    where nothing is differentiated; it may be the residual. Rows may be a strided view; anything else is copied first."""
+    return _native().linear(x, weight, bias, activation, residual, out)
 
 
 def norm_residual(x, block=None, *, gate=None, scale=1.0, post_weight=None, pre_weight=None, eps=1e-6):
@@ -215,27 +56,7 @@ def norm_residual(x, block=None, *, gate=None, scale=1.0, post_weight=None, pre_
     ``r`` is the residual stream behind the block, ``h`` what the next block reads. x, block ``[..., width]``; gate
     ``[width]`` or ``[..., width]`` or None (1); weights ``[width]`` or None (1); width 1 ... 4096. Without a block
     ``r = x``. Differentiable (once) in all five tensors; scale and eps are numbers."""
-    _check_x(x)
-    if x.dim() < 1:
-        raise ValueError("x must be [..., width]")
-    lead, width = x.shape[:-1], x.shape[-1]
-    if not 1 <= width <= 4096:
-        raise ValueError(f"width must be 1 ... 4096, got {width}")
-    _check("block", block, x.shape, x)
-    _check("post_weight", post_weight, (width,), x)
-    _check("pre_weight", pre_weight, (width,), x)
-    if block is None and (gate is not None or post_weight is not None):
-        raise ValueError("gate and post_weight belong to a block")
-    if gate is not None:
-        _check("gate", gate, (width,) if gate.dim() == 1 and x.dim() > 1 else x.shape, x)
-    if not eps >= 0:
-        raise ValueError("eps must not be negative")
-    flat = None if gate is None else gate.contiguous() if gate.dim() == 1 and x.dim() > 1 else _rows(gate)
-    args = (_rows(x), _rows(block), flat, None if post_weight is None else post_weight.contiguous(),
-            None if pre_weight is None else pre_weight.contiguous(), float(scale), float(eps))
-    learn = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, block, gate, post_weight, pre_weight))
-    r, h = _NormFunction.apply(*args) if learn else _norm_forward(*args)
-    return r.view(*lead, width), h.view(*lead, width)
+    return _native().norm_residual(x, block, gate, scale, post_weight, pre_weight, eps)
 
 
 @torch.no_grad()
@@ -246,43 +67,16 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.
     params and grads of one type; exp_avgs, exp_avg_sqs float32; 16-bit params need float32 ``masters`` (the params are
     their rounded copies). ``step``: int32 tensor ``[1]`` on the device, the steps done so far; the call adds 1, so a step
     captured into a graph replays with an advancing count. All tensors contiguous, on one GPU, none twice."""
-    params = list(params)
-    if not params:
-        raise ValueError("no parameters")
-    first = params[0]
-    _check_x(first, "params[0]")
-    lists = [("grads", grads, first.dtype), ("exp_avgs", exp_avgs, torch.float32), ("exp_avg_sqs", exp_avg_sqs, torch.float32)]
-    if (masters is None) == (first.dtype != torch.float32):
-        raise ValueError("16-bit params need float32 masters, float32 params have none")
-    if masters is not None:
-        lists.append(("masters", masters, torch.float32))
-    seen = set()
-    for name, tensors, dtype in [("params", params, first.dtype), *lists]:
-        if len(tensors) != len(params):
-            raise ValueError(f"{len(tensors)} {name} for {len(params)} params")
-        for t, p in zip(tensors, params):
-            if t.dtype != dtype or t.device != first.device or t.shape != p.shape or not t.is_contiguous():
-                raise ValueError(f"{name}: expected a contiguous {dtype} tensor of shape {tuple(p.shape)} on {first.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-            if t.numel() and t.data_ptr() in seen:
-                raise ValueError(f"{name}: a tensor is there twice")
-            seen.add(t.data_ptr())
-    if step.dtype != torch.int32 or step.numel() != 1 or step.device != first.device:
-        raise ValueError("step must be an int32 tensor of one element on the params' device")
-    pack = abi.ADAMW_TENSOR.pack
-    table = b"".join([
-        pack(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), _ptr(w), p.numel())
-        for p, g, m, v, w in zip(params, grads, exp_avgs, exp_avg_sqs, masters or [None] * len(params))])
-    at = C.cast(table, C.c_void_p).value  # the table is read during the call
-    norm = torch.empty(1, dtype=torch.float32, device=first.device)
+    return _native().adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas, eps, weight_decay, max_grad_norm, masters)
 
-    def blob(work):
-        return abi.ADAMW_CALL.pack(
-            _ADAMW_SIZE, first.get_device(), _DTYPES[first.dtype], len(params), at, step.data_ptr(), norm.data_ptr(),
-            lr, betas[0], betas[1], eps, weight_decay, 0.0 if max_grad_norm is None else max_grad_norm, _ptr(work), 0 if work is None else work.numel())
 
-    work = _workspace("drone_adamw_workspace", blob(None), first.device)
-    _call("drone_adamw_step", blob(work), first.device)
-    return norm
+def _check_parameter(p):
+    if p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError(f"a parameter is {p.dtype}: float32, bfloat16 or float16")
+    if p.device.type != "cuda":
+        raise ValueError(f"a parameter is on {p.device}: the policy operators run on a GPU only")
+    if not p.is_contiguous():
+        raise ValueError("parameters must be contiguous")
 
 
 class AdamW(torch.optim.Optimizer):
@@ -301,11 +95,10 @@ class AdamW(torch.optim.Optimizer):
         for group in self.param_groups:
             if len({p.dtype for p in group["params"]}) != 1 or len({p.device for p in group["params"]}) != 1:
                 raise ValueError("the parameters of a group must have one type and one device")
-            _check_x(group["params"][0], "a parameter")
+            for p in group["params"]:
+                _check_parameter(p)
             group["step"] = torch.zeros(1, dtype=torch.int32, device=group["params"][0].device)
             for p in group["params"]:
-                if not p.is_contiguous():
-                    raise ValueError("parameters must be contiguous")
                 self.state[p] = {"exp_avg": torch.zeros(p.shape, dtype=torch.float32, device=p.device), "exp_avg_sq": torch.zeros(p.shape, dtype=torch.float32, device=p.device)}
                 if p.dtype != torch.float32:
                     self.state[p]["master"] = p.detach().float()

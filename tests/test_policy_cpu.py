@@ -9,13 +9,12 @@ import torch
 from drone_amd import abi, policy
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-STRUCTS = (("DroneLinear", abi.DroneLinear, abi.LINEAR_CALL), ("DroneNorm", abi.DroneNorm, abi.NORM_CALL),
-           ("DroneAdamWTensor", abi.DroneAdamWTensor, abi.ADAMW_TENSOR), ("DroneAdamW", abi.DroneAdamW, abi.ADAMW_CALL))
+STRUCTS = (("DroneLinear", abi.DroneLinear), ("DroneNorm", abi.DroneNorm), ("DroneAdamWTensor", abi.DroneAdamWTensor), ("DroneAdamW", abi.DroneAdamW))
 
 
 def test_call_structs_match_the_header(tmp_path):
     lines = []
-    for name, cls, _ in STRUCTS:
+    for name, cls in STRUCTS:
         lines.append(f'printf("{name} %zu\\n", sizeof({name}));')
         lines += [f'printf("{name}.{f} %zu\\n", offsetof({name}, {f}));' for f, _t in cls._fields_]
     lines += [f'printf("{n} %d\\n", {n});' for n in ("DRONE_F32", "DRONE_BF16", "DRONE_F16")]
@@ -23,16 +22,10 @@ def test_call_structs_match_the_header(tmp_path):
     (tmp_path / "l.c").write_text('#include <stdio.h>\n#include "drone_vec.h"\nint main(void){' + "".join(lines) + "return 0;}")
     subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(tmp_path / "l.c"), "-o", str(tmp_path / "l")], check=True)
     got = {k: int(v) for k, v in (l.split() for l in subprocess.run([str(tmp_path / "l")], check=True, capture_output=True, text=True).stdout.splitlines())}
-    for name, cls, fmt in STRUCTS:
-        assert got[name] == C.sizeof(cls) == fmt.size, name
+    for name, cls in STRUCTS:
+        assert got[name] == C.sizeof(cls), name
         for f, _t in cls._fields_:
             assert got[f"{name}.{f}"] == getattr(cls, f).offset, f"{name}.{f}"
-        # the packed form names the same fields in the same places
-        values = list(range(1, len(cls._fields_) + 1))
-        back = cls.from_buffer_copy(fmt.pack(*values))
-        for (f, _t), want in zip(cls._fields_, values):
-            v = getattr(back, f)
-            assert (C.cast(v, C.c_void_p).value if f == "tensors" else v) == want, f"{name}.{f}"
     assert (got["DRONE_F32"], got["DRONE_BF16"], got["DRONE_F16"]) == (abi.F32, abi.BF16, abi.F16)
     assert {n.lower(): got[f"DRONE_ACTIVATION_{n}"] for n in ("NONE", "RELU", "TANH", "SILU", "GELU")} == abi.ACTIVATIONS
 
@@ -124,7 +117,15 @@ def test_empty_calls_do_nothing(hip):
     assert f["drone_linear_backward"](C.byref(linear_call(dx=None, dweight=None, dbias=None)), None) == 0
 
 
-def test_cpu_tensors_are_refused():
+@pytest.fixture(scope="module")
+def native(hip):
+    """The compiled module (bindings/policy_torch.cpp): git-ignored like the library, built where it is missing."""
+    if not any(f.startswith("policy_torch") for f in os.listdir(os.path.join(ROOT, "drone_amd"))):
+        subprocess.run(["make", "-C", os.path.join(ROOT, "bindings")], check=True, capture_output=True)
+    return policy._native()
+
+
+def test_cpu_tensors_are_refused(native):
     x, w = torch.zeros(4, 8), torch.zeros(3, 8)
     with pytest.raises(ValueError, match="GPU only"):
         policy.linear(x, w)
