@@ -19,52 +19,47 @@ constexpr int kJoinThreads = 256;
 
 template <class T> __device__ __forceinline__ float to_f(T v) { return (float)v; }
 
-// ---- activation: value and slope in 32 bits, by the hardware's exp2 and rcp (1 ulp each). tanh and silu keep a relative
-// error of about 1e-6 everywhere (tanh by its series near zero, its slope from 1 - |a|, not from 1 - a^2). erf: the math
-// library's for f32 tensors; Abramowitz & Stegun 7.1.26 (|error| <= 1.5e-7) for the 16-bit types, whose exp(-z^2/2) is
-// also what the slope needs. ----
+// ---- activation: value and slope in 32 bits, by the hardware's exp2 and rcp (1 ulp each). f32 tensors: tanh by its series
+// near zero and erf from the math library. 16-bit tensors: absolute errors of 2e-7 are far below the result's rounding, and the
+// instructions count (the epilogue of a narrow layer is as long as its product): tanh = 1 - 2 / (1 + exp 2z), erfc by
+// Abramowitz & Stegun 7.1.26 (|error| <= 1.5e-7), whose exp(-z^2/2) is also what the slope needs. The forms are chosen so that
+// infinities give the limits (no 0 * inf) and NaNs stay. ----
 template <int ACT, bool PRECISE>
 __device__ __forceinline__ float activate(float z, float& slope) {
     switch (ACT) {
         case DRONE_ACTIVATION_RELU:
             slope = z > 0.f ? 1.f : 0.f;
-            return z > 0.f ? z : (z != z ? z : 0.f);  // a NaN stays one
+            return z > 0.f ? z : (z != z ? z : 0.f);
         case DRONE_ACTIVATION_TANH: {
-            const float x = 2.f * __builtin_amdgcn_rcpf(1.f + __expf(2.f * fabsf(z)));  // 1 - |tanh z|
-            const float q = z * z;
-            const float series = z * (1.f + q * (-0.33333334f + q * (0.13333334f + q * (-0.05396825f + q * 0.02186949f))));
-            const bool small = q < 0.0625f;  // the series' next term is 1e-8 of z there
-            slope = small ? 1.f - series * series : x * (2.f - x);
-            return small ? series : copysignf(1.f - x, z);
+            if (PRECISE) {
+                const float x = 2.f * __builtin_amdgcn_rcpf(1.f + __expf(2.f * fabsf(z)));  // 1 - |tanh z|
+                const float q = z * z;
+                const float series = z * (1.f + q * (-0.33333334f + q * (0.13333334f + q * (-0.05396825f + q * 0.02186949f))));
+                const bool small = q < 0.0625f;  // the series' next term is 1e-8 of z there
+                slope = small ? 1.f - series * series : x * (2.f - x);
+                return small ? series : copysignf(1.f - x, z);
+            }
+            const float r = __builtin_amdgcn_rcpf(1.f + __expf(2.f * z));
+            slope = 4.f * r * (1.f - r);
+            return 1.f - 2.f * r;
         }
         case DRONE_ACTIVATION_SILU: {
-            const float s = __builtin_amdgcn_rcpf(1.f + __expf(-z));
-            slope = s * (1.f + z * (1.f - s));
-            if (fabsf(z) > 80.f) {  // 0 * inf at the infinities: the limits instead
-                slope = z > 0.f ? 1.f : 0.f;
-                return z > 0.f ? z : 0.f;
-            }
-            return z * s;
+            const float s = __builtin_amdgcn_rcpf(1.f + __expf(-z)), c = fminf(fmaxf(z, -90.f), 90.f);
+            slope = s + c * (s * (1.f - s));
+            return z < -90.f ? 0.f : z * s;
         }
-        case DRONE_ACTIVATION_GELU: {
+        case DRONE_ACTIVATION_GELU: {  // max(z, 0) - |z| Q(|z|), Q(x) = 1/2 erfc(x / sqrt 2)
             const float e = __expf(-0.5f * z * z);
-            float cdf;
+            float tail;
             if (PRECISE) {
-                cdf = 0.5f * (1.f + erff(z * 0.70710678f));
+                tail = 0.5f * erfcf(fabsf(z) * 0.70710678f);
             } else {
-                const float x = fabsf(z) * 0.70710678f;
-                const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * x);
-                const float p = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-                const float half_tail = 0.5f * p * e;
-                cdf = z >= 0.f ? 1.f - half_tail : half_tail;
+                const float t = __builtin_amdgcn_rcpf(1.f + 0.23164189f * fabsf(z));
+                tail = e * (t * (0.127414796f + t * (-0.142248368f + t * (0.7107068705f + t * (-0.7265760135f + t * 0.5307027145f)))));
             }
-            const float pdf = e * 0.39894228f;
-            if (fabsf(z) > 3e38f) {  // an infinity: 0 * inf below
-                slope = z > 0.f ? 1.f : 0.f;
-                return z > 0.f ? z : 0.f;
-            }
-            slope = cdf + z * pdf;
-            return z * cdf;
+            const float c = fminf(fmaxf(z, -30.f), 30.f);
+            slope = (z < 0.f ? tail : 1.f - tail) + c * (e * 0.39894228f);
+            return fmaxf(z, 0.f) - fminf(fabsf(z), 30.f) * tail;
         }
         default:
             slope = 1.f;
@@ -108,10 +103,14 @@ __device__ __forceinline__ void store_n(S* p, long long left, const float* f) {
 __device__ __forceinline__ int swz(int r) { return (r ^ (r >> 3)) & 7; }
 
 // The matrix instruction leaves a lane the result rows 8 a + 4 half + b (a, b = 0 ... 3) of its first operand. The features
-// are that operand, and feature 16 half + 4 a + b of every 32 is put into that row, so a lane owns 16 neighbouring features
-// of one output row: 32- or 64-byte pieces instead of 8- or 16-byte ones.
-__device__ __forceinline__ int feature_of(int i) { return (i & ~31) | ((i & 4) << 2) | ((i & 24) >> 1) | (i & 3); }
-__device__ __forceinline__ int row_of_feature(int f) { return (f & ~31) | ((f & 16) >> 2) | ((f & 12) << 1) | (f & 3); }
+// are that operand. f32: in their order, four neighbours are a 16-byte piece and the two halves of the wave hold neighbouring
+// pieces. 16-bit types: feature 16 half + 4 a + b of every 32 is put into that row, so that a lane owns 16 neighbours, 32
+// bytes of one output row (262144 x 256 x 256 bf16: 133 us; pieces of 8 interleaved between the halves: 148; f32 the other way
+// round, 65536 x 64 x 64: 23 against 17 us).
+template <class T> __device__ __forceinline__ int feature_of(int i) { return sizeof(T) == 4 ? i : (i & ~31) | ((i & 4) << 2) | ((i & 24) >> 1) | (i & 3); }
+template <class T> __device__ __forceinline__ int row_of_feature(int f) { return sizeof(T) == 4 ? f : (f & ~31) | ((f & 16) >> 2) | ((f & 12) << 1) | (f & 3); }
+// The lane's q-th piece of 32 features begins here (registers q kE ... of its sixteen).
+template <class T> __device__ __forceinline__ int piece_feature(int q, int half) { return sizeof(T) == 4 ? (2 * q + half) * 4 : half * 16 + q * 8; }
 
 // One operand as it lies in memory. CONTIG tiles: [row][reduction]; the others: [reduction][row]. With `slope` (a dense
 // companion) the element is v * slope: the dz of the gradient, formed in 32 bits and rounded once for the matrix core.
@@ -139,7 +138,7 @@ struct ContigTile {
         const long long k = k0 + (threadIdx.x & 7) * kE, left = WHOLE ? kE : kend - k;
 #pragma unroll
         for (int i = 0; i < kN; i++) {
-            long long r = row0 + (FEATURES ? feature_of(lds_row(i)) : lds_row(i));
+            long long r = row0 + (FEATURES ? feature_of<T>(lds_row(i)) : lds_row(i));
             r = r < rows ? r : rows - 1;
             if (left <= 0) {
 #pragma unroll
@@ -209,7 +208,7 @@ struct TransTile {
         for (int i = 0; i < kN; i++) {
             const int b = threadIdx.x + i * THREADS;
             if (kBlocks % THREADS && b >= kBlocks) break;
-            const int r = (b % (ROWS / 4)) * 4, c = b / (ROWS / 4), at = FEATURES ? row_of_feature(r) : r;
+            const int r = (b % (ROWS / 4)) * 4, c = b / (ROWS / 4), at = FEATURES ? row_of_feature<T>(r) : r;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 Vec<T, kE> v;
@@ -253,7 +252,7 @@ __device__ __forceinline__ Unit unit_of(long long tiles, int tiles_n, long long 
     return r;
 }
 
-// What a lane does with its results: 16 neighbouring features of row row0 + 32 m + lane % 32 for each (n, m). Everything the
+// What a lane does with its results: 16 features (piece_feature) of row row0 + 32 m + lane % 32 for each (n, m). Everything the
 // epilogue reads is asked for before the first value is used.
 template <class T, int ACT, int TM, int TN, bool WHOLE>
 __device__ __forceinline__ void write_forward(const LinearArgs& a, const f32x16 (&acc)[TN][TM], long long row0, long long feat0) {
@@ -262,7 +261,7 @@ __device__ __forceinline__ void write_forward(const LinearArgs& a, const f32x16 
     const int half = (threadIdx.x >> 5) & 1, l32 = threadIdx.x & 31;
     u32x4 b[TN][kQ], res[TM][TN][kQ];  // as they come: unpacked where they are used
     using Piece = Vec<T, kE>;
-    auto feat_of = [&](int n, int q) { return feat0 + n * 32 + half * 16 + q * kE; };  // register r of a lane: feature 16 half + r
+    auto feat_of = [&](int n, int q) { return feat0 + n * 32 + piece_feature<T>(q, half); };
     auto left_of = [&](int n, int q) { return WHOLE ? (long long)kE : a.out - feat_of(n, q); };
 #pragma unroll
     for (int n = 0; n < TN; n++)
@@ -335,7 +334,7 @@ __device__ __forceinline__ void write_results(const LinearArgs& a, const f32x16 
                 for (int n = 0; n < TN; n++)
 #pragma unroll
                     for (int q = 0; q < 16 / kE; q++) {
-                        const long long feat = feat0 + n * 32 + half * 16 + q * kE, left = kWhole ? kE : nfeat - feat;
+                        const long long feat = feat0 + n * 32 + piece_feature<T>(q, half), left = kWhole ? kE : nfeat - feat;
                         if (left <= 0) continue;
                         float v[kE];
 #pragma unroll
@@ -479,7 +478,7 @@ struct StreamTile {
                 f = f < rows ? f : rows - kE;  // past the end: any piece of the row, its results are not stored
                 base[i] = p + m * ld + f;
             } else {
-                long long r = row0 + (FEATURES ? feature_of(s / PIECES) : s / PIECES);
+                long long r = row0 + (FEATURES ? feature_of<T>(s / PIECES) : s / PIECES);
                 r = r < rows ? r : rows - 1;
                 base[i] = p + r * ld + offset(i);
             }
@@ -509,7 +508,7 @@ struct StreamTile {
             return lds[r * PIECES + ((2 * s + half) ^ piece_swz<PIECES>(r))];
         } else if constexpr (sizeof(T) == 2) {
             // sixteen lanes turn a block of four steps x 16 features: lane j points at step j / 4, features 4 (j % 4) ...
-            const int i = (lane & 16) + 4 * (lane & 3), f = block + (FEATURES ? feature_of(i) : i), m0 = (lane & 15) >> 2;
+            const int i = (lane & 16) + 4 * (lane & 3), f = block + (FEATURES ? feature_of<T>(i) : i), m0 = (lane & 15) >> 2;
             union { u32x4 u; s16x4 h[2]; } v;
 #pragma unroll
             for (int t = 0; t < 2; t++) {
@@ -519,7 +518,7 @@ struct StreamTile {
             }
             return v.u;
         } else {
-            const int f = block + (FEATURES ? feature_of(l32) : l32);
+            const int f = block + (FEATURES ? feature_of<T>(l32) : l32);
             u32x4 v;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
@@ -603,6 +602,153 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void linear_stream_kernel(LinearAr
         buf = buf == STAGES - 1 ? 0 : buf + 1;
     }
     write_results<T, P, TM, TN>(a, acc, row0 + wrow, nrows, feat0 + wfeat, nfeat, feat0 + BN <= nfeat, unit.part);
+}
+
+// ---- a reduction of at most 1 KiB a row (512 16-bit, 256 f32): the weights stay in registers, 32 features a wave, and rows
+// (with their residuals) stream through LDS. Persistent workgroups, all of LDS in row tiles under way, one barrier a tile:
+// a tile costs its bytes and little else, where the tiled form pays a load latency for each of its few reduction steps and
+// another for its epilogue. Loads into registers would spoil it: they retire in order behind the tiles under way, so the
+// first one waits for them all (262144 x 256 x 256 bf16 with the residual in registers: 240 us). ----
+constexpr int kResidentWaves = 8;
+
+// Weight fragments of one wave: step s holds the lane's 16 bytes of feature lane % 32 from reduction 32-byte step s on.
+template <class T, int KS>
+__device__ __forceinline__ void load_weights(u32x4 (&w)[KS], const T* p, long long ld, int feat0, int nfeat, int red) {
+    constexpr int kE = Elem<T>::kE;
+    const int lane = threadIdx.x & 63, half = lane >> 5, f = feat0 + feature_of<T>(lane & 31);
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+        const int k = (2 * s + half) * kE;
+        w[s] = u32x4{0, 0, 0, 0};
+        if (f < nfeat && k < red) w[s] = __builtin_bit_cast(u32x4, load_n<T, kE>(p + f * ld + k, red - k));
+    }
+}
+
+// ROWS rows of PIECES 16-byte pieces in LDS, piece p of row r at p ^ swizzle(r) (sixteen rows' same piece in different banks).
+template <class T, int ROWS, int PIECES>
+struct RowTile {
+    static constexpr int kE = Elem<T>::kE, kLoads = ROWS * PIECES / 64, kN = (kLoads + kResidentWaves - 1) / kResidentWaves;
+    __device__ __forceinline__ static int swizzle(int r) { return PIECES >= 16 ? r & 15 : PIECES == 8 ? (r >> 1) & 7 : (r >> 2) & 3; }
+    __device__ __forceinline__ static int at(int r, int piece) { return r * PIECES + (piece ^ swizzle(r)); }
+    // The wave's i-th load: with fewer loads than waves some repeat another's, so that every wave has the same number under way.
+    __device__ __forceinline__ static int load_of(int i) { return ((threadIdx.x >> 6) + i * kResidentWaves) % kLoads; }
+    __device__ __forceinline__ static int slot(int i) { return load_of(i) * 64 + (threadIdx.x & 63); }
+    __device__ __forceinline__ static int piece_of(int i) { return (slot(i) % PIECES) ^ swizzle(slot(i) / PIECES); }
+    // Pieces past the row's end are never written: zero for good (a garbage x would make its product with a zero weight a NaN).
+    __device__ __forceinline__ static void clear(u32x4* lds, int pieces) {
+#pragma unroll
+        for (int i = 0; i < kN; i++) if (piece_of(i) >= pieces) lds[slot(i)] = u32x4{0, 0, 0, 0};
+    }
+    // Every load covers at least one whole row, so none of a wave's loads is ever skipped (landed() counts them).
+    static_assert(64 % PIECES == 0 || PIECES % 64 == 0, "whole rows");
+    __device__ __forceinline__ static void stage(u32x4* lds, const T* p, long long ld, long long row0, long long rows, int pieces) {
+#pragma unroll
+        for (int i = 0; i < kN; i++) {
+            const long long r0 = row0 + slot(i) / PIECES, r = r0 < rows ? r0 : rows - 1;
+            const int piece = piece_of(i);
+            if (piece < pieces)
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(p + r * ld + piece * kE),
+                                                 (__attribute__((address_space(3))) void*)(lds + load_of(i) * 64), 16, 0, 0);
+        }
+    }
+};
+
+template <class T, int KS, int WF, bool RES>
+struct Resident {
+    static constexpr int kE = Elem<T>::kE, kQ = 16 / kE, kRows = kResidentWaves / WF * 32;
+    using X = RowTile<T, kRows, 2 * KS>;
+    using R = RowTile<T, kRows, WF * 32 / kE>;
+    static constexpr int kX = kRows * 2 * KS, kTile = kX + (RES ? kRows * WF * 32 / kE : 0);  // pieces
+    // Tiles of LDS: two workgroups a CU where the registers allow it (short reductions), else one with most of the memory.
+    static constexpr int kPerCu = KS <= 4 && kTile * 16 * 4 <= 72 * 1024 ? 2 : 1, kFit = 144 * 1024 / kPerCu / (kTile * 16), kStages = kFit > 8 ? 8 : kFit;
+    static constexpr int kLoads = X::kN + (RES ? R::kN : 0);  // a wave's for one tile
+    static_assert(kStages >= 2, "at least one tile ahead");
+};
+
+template <class T, int ACT, int KS, int WF, bool RES, bool SLOPE>
+__device__ __forceinline__ void resident_forward(const LinearArgs& a, u32x4 (*lds)[Resident<T, KS, WF, RES>::kTile], int groups, int slots) {
+    using M = Resident<T, KS, WF, RES>;
+    using Slope = typename Elem<T>::Slope;
+    constexpr int kE = M::kE, kQ = M::kQ, kBM = M::kRows, kStages = M::kStages;
+    constexpr int kStores = kQ + (SLOPE ? kQ * kE * (int)sizeof(Slope) / 16 : 0);  // a wave's for one tile
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, r = (wave / WF) * 32 + (lane & 31);
+    const int xcd = blockIdx.x & 7, at = blockIdx.x >> 3, group = at % groups, pieces = a.in / kE;
+    const int tiles = (int)((a.rows + kBM - 1) / kBM), step = 8 * slots, group0 = group * WF * 32, feat0 = group0 + wave % WF * 32;
+    int tile = xcd * slots + at / groups;
+    if (tile >= tiles) return;
+    auto stage = [&](int to, int t) {
+        M::X::stage(lds[to], (const T*)a.x, a.x_ld, (long long)t * kBM, a.rows, pieces);
+        if (RES) M::R::stage(lds[to] + M::kX, (const T*)a.res + group0, a.res_ld, (long long)t * kBM, a.rows, (a.out - group0) / kE);
+    };
+#pragma unroll
+    for (int i = 0; i < kStages; i++) M::X::clear(lds[i], pieces);
+    u32x4 w[KS], bias[kQ];
+    load_weights<T, KS>(w, (const T*)a.w, a.w_ld, feat0, a.out, a.in);
+    auto left = [&](int q) { return a.out - feat0 - piece_feature<T>(q, half); };
+    auto column = [&](int q) { return feat0 + piece_feature<T>(q, half); };
+#pragma unroll
+    for (int q = 0; q < kQ; q++) {
+        bias[q] = u32x4{0, 0, 0, 0};
+        if (a.b && left(q) > 0) bias[q] = __builtin_bit_cast(u32x4, load_n<T, kE>((const T*)a.b + column(q), left(q)));
+    }
+#pragma unroll
+    for (int i = 0; i < kStages - 1; i++)
+        if (tile + i * step < tiles) stage(i, tile + i * step);
+    const bool whole = feat0 + 32 <= a.out;  // the wave's stores all go out (its rows are whole up to the last tile)
+    int buf = 0;
+    for (int turn = 0; tile < tiles; tile += step, turn++) {
+        // this tile's loads have kStages - 2 tiles' behind them, and from the kStages-th turn on as many tiles' stores and one more
+        if (tile + (kStages - 2) * step >= tiles) landed<0>();
+        else if (whole && turn >= kStages - 1) landed<((kStages - 2) * M::kLoads + (kStages - 1) * kStores < 63 ? (kStages - 2) * M::kLoads + (kStages - 1) * kStores : 63)>();
+        else landed<(kStages - 2) * M::kLoads>();
+        const int next = buf == 0 ? kStages - 1 : buf - 1;
+        if (tile + (kStages - 1) * step < tiles) stage(next, tile + (kStages - 1) * step);
+        f32x16 acc;
+#pragma unroll
+        for (int q = 0; q < kQ; q++) {
+            const auto b = __builtin_bit_cast(Vec<T, kE>, bias[q]);
+#pragma unroll
+            for (int j = 0; j < kE; j++) acc[q * kE + j] = to_f(b.e[j]);
+        }
+#pragma unroll
+        for (int s = 0; s < KS; s++) mfma(acc, w[s], lds[buf][M::X::at(r, 2 * s + half)], T{});
+        const long long row = (long long)tile * kBM + r;
+        auto write = [&](auto is_whole) {
+#pragma unroll
+            for (int q = 0; q < kQ; q++) {
+                const int n = decltype(is_whole)::value ? kE : left(q);
+                if (n <= 0) continue;
+                float v[kE], s[kE];
+#pragma unroll
+                for (int j = 0; j < kE; j++) v[j] = activate<ACT, sizeof(T) == 4>(acc[q * kE + j], s[j]);
+                if (SLOPE) store_n<Slope, kE>((Slope*)a.slope + row * a.out + column(q), n, s);
+                if (RES) {
+                    const auto more = __builtin_bit_cast(Vec<T, kE>, lds[buf][M::kX + M::R::at(r, (column(q) - group0) / kE)]);
+#pragma unroll
+                    for (int j = 0; j < kE; j++) v[j] += to_f(more.e[j]);
+                }
+                store_n<T, kE>((T*)a.y + row * a.y_ld + column(q), n, v);
+            }
+        };
+        if (row < a.rows) { if (whole) write(std::true_type{}); else write(std::false_type{}); }
+        buf = buf == kStages - 1 ? 0 : buf + 1;
+    }
+}
+
+template <class T, int KS, int WF, bool RES, int PER_CU>
+__global__ __launch_bounds__(kResidentWaves * 64, 2 * PER_CU) void linear_resident_kernel(LinearArgs a, int groups, int slots) {
+    __shared__ u32x4 lds[Resident<T, KS, WF, RES>::kStages][Resident<T, KS, WF, RES>::kTile];
+    auto go = [&](auto act) {
+        if (a.slope) resident_forward<T, decltype(act)::value, KS, WF, RES, true>(a, lds, groups, slots);
+        else resident_forward<T, decltype(act)::value, KS, WF, RES, false>(a, lds, groups, slots);
+    };
+    switch (a.act) {
+        case DRONE_ACTIVATION_RELU: go(std::integral_constant<int, DRONE_ACTIVATION_RELU>{}); break;
+        case DRONE_ACTIVATION_TANH: go(std::integral_constant<int, DRONE_ACTIVATION_TANH>{}); break;
+        case DRONE_ACTIVATION_SILU: go(std::integral_constant<int, DRONE_ACTIVATION_SILU>{}); break;
+        case DRONE_ACTIVATION_GELU: go(std::integral_constant<int, DRONE_ACTIVATION_GELU>{}); break;
+        default: go(std::integral_constant<int, DRONE_ACTIVATION_NONE>{});
+    }
 }
 
 // dz = dy * slope, rounded once to T, into a dense [rows][out] buffer (or nowhere: dz is dy), and the bias gradient's partial
@@ -766,10 +912,58 @@ int backward_stream(LinearArgs a, hipStream_t s) {
     return (int)hipGetLastError();
 }
 
+// Persistent workgroups: as many as stay on the card at once, in whole multiples of the feature groups for each XCD.
+template <class T, int KS, int WF, bool RES>
+int resident(const LinearArgs& a, hipStream_t s) {
+    using M = Resident<T, KS, WF, RES>;
+    const int groups = (a.out + WF * 32 - 1) / (WF * 32);
+    const long long tiles = (a.rows + M::kRows - 1) / M::kRows;
+    long long slots = 32 * M::kPerCu / groups;  // row tiles in work on each XCD
+    if (slots < 1) slots = 1;
+    // With fewer than eight tiles each there is nothing to keep under way (65536 x 64 x 64 f32, two tiles a workgroup: 21.6 us
+    // against 16.8 of the tiled form; 262144 x 256 x 256 bf16, thirty-two: 101 against 133).
+    if (tiles < 64 * slots) return -1;
+    linear_resident_kernel<T, KS, WF, RES, M::kPerCu><<<(unsigned)(8 * slots * groups), kResidentWaves * 64, 0, s>>>(a, groups, (int)slots);
+    return (int)hipGetLastError();
+}
+
+template <class T, int KS, bool RES>
+int resident_wide(const LinearArgs& a, hipStream_t s) {
+    if constexpr (KS <= 4) {
+        if (a.out <= 32) return resident<T, KS, 1, RES>(a, s);
+    }
+    if constexpr (KS <= 8) {
+        if (a.out <= 64) return resident<T, KS, 2, RES>(a, s);
+    }
+    if constexpr (KS <= 16) {
+        if (a.out <= 128) return resident<T, KS, 4, RES>(a, s);
+    }
+    return resident<T, KS, 8, RES>(a, s);
+}
+
+template <class T>
+int resident_any(const LinearArgs& a, hipStream_t s) {
+    const int steps = (a.in / Elem<T>::kE + 1) / 2;
+    auto go = [&](auto res) {
+        constexpr bool kRes = decltype(res)::value;
+        if (steps <= 4) return resident_wide<T, 4, kRes>(a, s);
+        if (steps <= 8) return resident_wide<T, 8, kRes>(a, s);
+        if (steps <= 16) return resident_wide<T, 16, kRes>(a, s);
+        return resident_wide<T, 32, kRes>(a, s);
+    };
+    return a.res ? go(std::true_type{}) : go(std::false_type{});
+}
+
 template <class T>
 int forward_any(const LinearArgs& a, hipStream_t s) {
     constexpr int kE = Elem<T>::kE;
-    if (a.in % kE == 0 && a.x_ld % kE == 0 && a.w_ld % kE == 0 && aligned16(a.x) && aligned16(a.w) && a.out > 32 && !few(a.rows, a.out)) return stream_product<T, kForward>(a, a.out, s);
+    const bool pieces = a.in % kE == 0 && a.x_ld % kE == 0 && a.w_ld % kE == 0 && aligned16(a.x) && aligned16(a.w);
+    const bool whole_res = !a.res || (a.out % kE == 0 && a.res_ld % kE == 0 && aligned16(a.res));
+    if (pieces && whole_res && a.in * (int)sizeof(T) <= 1024) {
+        const int rc = resident_any<T>(a, s);
+        if (rc >= 0) return rc;
+    }
+    if (pieces && a.out > 32 && !few(a.rows, a.out)) return stream_product<T, kForward>(a, a.out, s);
     return product<T, kForward>(a, a.out, s);
 }
 
