@@ -98,6 +98,33 @@ __device__ __forceinline__ void store_n(S* p, long long left, const float* f) {
     }
 }
 
+// Elements at ... at + N - 1 of a row of `end` elements, zero past its end, without a branch (a branch around each load of a
+// tile makes the loads wait for one another) and without touching what lies behind the row: the last N elements, shifted.
+template <class S, int N>
+__device__ __forceinline__ Vec<S, N> load_end(const S* row, long long at, long long end) {
+    if constexpr (sizeof(S) * N > 16) {
+        const auto lo = load_end<S, N / 2>(row, at, end), hi = load_end<S, N / 2>(row, at + N / 2, end);
+        Vec<S, N> v;
+#pragma unroll
+        for (int e = 0; e < N / 2; e++) { v.e[e] = lo.e[e]; v.e[N / 2 + e] = hi.e[e]; }
+        return v;
+    } else {
+        using Bits = std::conditional_t<sizeof(S) * N == 16, unsigned __int128, uint64_t>;
+        using Pack = Vec<S, N>;
+        Bits bits = 0;
+        if (end >= N) {  // the same for the launch
+            const long long from = at < end - N ? at : end - N, shift = at - from;
+            __builtin_memcpy(&bits, row + from, sizeof(bits));
+            bits = shift >= N ? 0 : bits >> (int)(shift * sizeof(S) * 8);
+            return __builtin_bit_cast(Pack, bits);
+        }
+        Vec<S, N> v;
+#pragma unroll
+        for (int e = 0; e < N; e++) v.e[e] = at + e < end ? row[at + e] : (S)0.f;
+        return v;
+    }
+}
+
 // ---- tiles in LDS: [row][8 pieces of 16 B], piece p of row r at p ^ swz(r): eight neighbouring rows read the same piece
 // from eight different bank groups, and the transposing loader's lanes (four rows apart) write to eight as well ----
 __device__ __forceinline__ int swz(int r) { return (r ^ (r >> 3)) & 7; }
@@ -132,22 +159,18 @@ struct ContigTile {
     __device__ __forceinline__ void load(const Operand<T>& o, long long row0, long long rows, long long k0, long long kend) {
         if (k0 + kPieces * kE <= kend) some<true>(o, row0, rows, k0, kend); else some<false>(o, row0, rows, k0, kend);
     }
-    // WHOLE: no piece of the tile crosses the end (the same for the workgroup), so the loads go out without a branch between
+    // WHOLE: no piece of the tile crosses the end (the same for the workgroup)
     template <bool WHOLE>
     __device__ __forceinline__ void some(const Operand<T>& o, long long row0, long long rows, long long k0, long long kend) {
-        const long long k = k0 + (threadIdx.x & 7) * kE, left = WHOLE ? kE : kend - k;
+        const long long k = k0 + (threadIdx.x & 7) * kE;
 #pragma unroll
         for (int i = 0; i < kN; i++) {
             long long r = row0 + (FEATURES ? feature_of<T>(lds_row(i)) : lds_row(i));
             r = r < rows ? r : rows - 1;
-            if (left <= 0) {
-#pragma unroll
-                for (int e = 0; e < kE; e++) reg[i].e[e] = (T)0.f;
-                continue;
-            }
-            reg[i] = load_n<T, kE>(o.p + r * o.ld + k, left);
+            reg[i] = WHOLE ? load_n<T, kE>(o.p + r * o.ld + k, kE) : load_end<T, kE>(o.p + r * o.ld, k, kend);
             if (o.slope) {
-                const auto q = load_n<typename Elem<T>::Slope, kE>(o.slope + r * o.slope_ld + k, left);
+                using S = typename Elem<T>::Slope;
+                const auto q = WHOLE ? load_n<S, kE>(o.slope + r * o.slope_ld + k, kE) : load_end<S, kE>(o.slope + r * o.slope_ld, k, kend);
 #pragma unroll
                 for (int e = 0; e < kE; e++) reg[i].e[e] = (T)(to_f(reg[i].e[e]) * to_f(q.e[e]));
             }
@@ -163,42 +186,46 @@ struct ContigTile {
 };
 
 // Holds the same tile from a [reduction][row] operand: a thread takes kE reduction steps x 4 rows (kE loads of 4 elements)
-// and turns them in registers, so the LDS tile and the fragment reads are those of the contiguous form.
+// and turns them in registers, so the LDS tile and the fragment reads are those of the contiguous form. A tile with fewer
+// blocks than threads is the work of whole waves (the features' from the last wave down, so that two small tiles share out).
 template <class T, int ROWS, int THREADS, bool FEATURES>
 struct TransTile {
     static constexpr int kE = Elem<T>::kE, kBlocks = ROWS / 4 * kPieces, kN = (kBlocks + THREADS - 1) / THREADS;
+    static_assert(kBlocks % THREADS == 0 || (kBlocks < THREADS && kBlocks % 64 == 0), "whole waves");
     Vec<T, 4> reg[kN][kE];
+    static __device__ __forceinline__ int block_of(int i) { return FEATURES ? THREADS - 1 - (int)threadIdx.x + i * THREADS : (int)threadIdx.x + i * THREADS; }
+    static __device__ __forceinline__ bool idle(int b) { return kBlocks < THREADS && b >= kBlocks; }
     // add: the 32-bit dz of this thread's four rows is added up over the reduction (the bias gradient)
     __device__ __forceinline__ void load(const Operand<T>& o, long long row0, long long rows, long long k0, long long kend, bool add, float (&sum)[kN][4]) {
         if (k0 + kPieces * kE <= kend && row0 + ROWS <= rows) some<true>(o, row0, rows, k0, kend, add, sum); else some<false>(o, row0, rows, k0, kend, add, sum);
     }
     template <bool WHOLE>
     __device__ __forceinline__ void some(const Operand<T>& o, long long row0, long long rows, long long k0, long long kend, bool add, float (&sum)[kN][4]) {
+        using S = typename Elem<T>::Slope;
 #pragma unroll
         for (int i = 0; i < kN; i++) {
-            const int b = threadIdx.x + i * THREADS;
-            const long long r = row0 + (b % (ROWS / 4)) * 4, k = k0 + b / (ROWS / 4) * kE, left = WHOLE ? 4 : rows - r;
-            const bool mine = kBlocks % THREADS == 0 || b < kBlocks;
+            const int b = block_of(i);
+            if (idle(b)) continue;
+            const long long r = row0 + (b % (ROWS / 4)) * 4, k = k0 + b / (ROWS / 4) * kE;
 #pragma unroll
             for (int e = 0; e < kE; e++) {
-                Vec<T, 4> v;
+                const bool in = WHOLE || k + e < kend;
+                const long long at = in ? k + e : kend - 1;  // steps past the end: the last one's values, put to zero below
+                Vec<T, 4> v = WHOLE ? load_n<T, 4>(o.p + at * o.ld + r, 4) : load_end<T, 4>(o.p + at * o.ld, r, rows);
+                float f[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) v.e[j] = (T)0.f;
-                if (mine && (WHOLE || (k + e < kend && left > 0))) {
-                    v = load_n<T, 4>(o.p + (k + e) * o.ld + r, left);
-                    if (o.slope) {
-                        const auto q = load_n<typename Elem<T>::Slope, 4>(o.slope + (k + e) * o.slope_ld + r, left);
+                for (int j = 0; j < 4; j++) f[j] = to_f(v.e[j]);
+                if (o.slope) {
+                    const auto q = WHOLE ? load_n<S, 4>(o.slope + at * o.slope_ld + r, 4) : load_end<S, 4>(o.slope + at * o.slope_ld, r, rows);
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const float f = to_f(v.e[j]) * to_f(q.e[j]);
-                            if (add) sum[i][j] += f;
-                            v.e[j] = (T)f;
-                        }
-                    } else if (add) {
-#pragma unroll
-                        for (int j = 0; j < 4; j++) sum[i][j] += to_f(v.e[j]);
-                    }
+                    for (int j = 0; j < 4; j++) { f[j] *= to_f(q.e[j]); v.e[j] = (T)f[j]; }
                 }
+                if (!WHOLE)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) { f[j] = in ? f[j] : 0.f; v.e[j] = in ? v.e[j] : (T)0.f; }
+                if (add)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) sum[i][j] += f[j];
                 reg[i][e] = v;
             }
         }
@@ -206,8 +233,8 @@ struct TransTile {
     __device__ __forceinline__ void store(u32x4* lds) const {
 #pragma unroll
         for (int i = 0; i < kN; i++) {
-            const int b = threadIdx.x + i * THREADS;
-            if (kBlocks % THREADS && b >= kBlocks) break;
+            const int b = block_of(i);
+            if (idle(b)) continue;
             const int r = (b % (ROWS / 4)) * 4, c = b / (ROWS / 4), at = FEATURES ? row_of_feature<T>(r) : r;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
@@ -393,7 +420,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void linear_kernel(LinearArgs a, i
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l32 = lane & 31;
     const int wrow = (wave / WN) * TM * 32, wfeat = (wave % WN) * TN * 32;
 
-    fetch(red0);
+    if (red0 < red1) fetch(red0);
     int buf = 0;
     for (long long k = red0; k < red1; k += kK) {
         rt.store(lds[buf]);
@@ -838,13 +865,13 @@ int product(const LinearArgs& a, long long feats, hipStream_t s) {
 }
 
 // The weight gradient's reduction over the rows is split into parts: enough workgroups to fill the 256 CUs (twice, unless
-// the product is so small that joining the parts costs more than it), at least 256 rows each.
+// the product is so small that joining the parts costs more than it), at least 128 rows each.
 struct Split { int bm, bn, parts; };
 Split split_of(long long rows, int in, int out) {
     Split r = {out <= 64 ? 64 : 128, in <= 64 ? 64 : 128, 1};
     const long long tiles = (long long)((out + r.bm - 1) / r.bm) * ((in + r.bn - 1) / r.bn), want = tiles <= 2 ? 256 : 512;
     long long parts = (want + tiles - 1) / tiles;
-    const long long most = (rows + 255) / 256;
+    const long long most = (rows + 127) / 128;
     if (parts > most) parts = most;
     r.parts = parts < 1 ? 1 : (int)parts;
     return r;

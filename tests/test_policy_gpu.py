@@ -102,6 +102,16 @@ def test_linear_shapes(t, m, k, n):
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m, k, n", [(66001, 256, 256), (66001, 512, 264), (66001, 136, 200), (66001, 40, 136), (140001, 128, 100), (140001, 64, 128), (270001, 72, 64), (530001, 24, 8), (530001, 32, 48),
+                                     (9001, 1024, 520), (20001, 520, 384), (9001, 333, 259), (70001, 20, 7)])
+@pytest.mark.parametrize("act, res", [("silu", True), ("gelu", False)])
+def test_linear_many_rows(t, m, k, n, act, res):
+    """Row counts at which the streaming forms run (weights in registers, tiles from memory to LDS, dz in a pass of its own),
+    with a last tile that is not whole, for reductions and feature counts of every class; unaligned widths keep theirs."""
+    check_linear(*linear_case(m, k, n, t, act, True, res), act, f"{m}x{k}x{n}")
+
+
+@pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("act", list(ACTS))
 @pytest.mark.parametrize("bias, res", [(True, False), (False, True), (False, False)])
 def test_linear_activations(t, act, bias, res):
