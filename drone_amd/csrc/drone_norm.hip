@@ -16,21 +16,30 @@ namespace drone {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kGradBlocks = 512;  // workgroups of the backward pass at most: each leaves one partial sum per column
+constexpr int kJoinThreads = 1024;
+constexpr int kGradBlocks = 1024;  // workgroups of the backward pass at most: each leaves one partial sum per column
 
+// kE neighbouring elements as they lie in memory, zero past the row's end.
 template <class T, bool VEC>
-__device__ __forceinline__ void load_piece(const T* p, int c, int width, float* f) {
+__device__ __forceinline__ u32x4 load_piece(const T* p, int c, int width) {
     constexpr int kE = Elem<T>::kE;
+    union { u32x4 u; T e[kE]; } v;
+    v.u = u32x4{0, 0, 0, 0};
     if (VEC) {
-        union { u32x4 u; T e[kE]; } v;
-        v.u = u32x4{0, 0, 0, 0};
         if (c < width) v.u = *(const u32x4*)(p + c);
-#pragma unroll
-        for (int e = 0; e < kE; e++) f[e] = (float)v.e[e];
     } else {
 #pragma unroll
-        for (int e = 0; e < kE; e++) f[e] = c + e < width ? (float)p[c + e] : 0.f;
+        for (int e = 0; e < kE; e++) if (c + e < width) v.e[e] = p[c + e];
     }
+    return v.u;
+}
+
+template <class T>
+__device__ __forceinline__ void unpack(u32x4 u, float* f) {
+    union { u32x4 u; T e[Elem<T>::kE]; } v;
+    v.u = u;
+#pragma unroll
+    for (int e = 0; e < Elem<T>::kE; e++) f[e] = (float)v.e[e];
 }
 
 template <class T, bool VEC>
@@ -47,11 +56,23 @@ __device__ __forceinline__ void store_piece(T* p, int c, int width, const float*
     }
 }
 
-// Sum over the TPR threads of a row, the same in all of them. 256: through LDS (`join`, 4 floats), two barriers.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ float plus_dpp(float v) {
+    return v + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, ROWS, 0xf, false));
+}
+
+// Sum over the TPR threads of a row, the same in all of them: neighbours' registers (a shuffle through LDS for each of six
+// steps, four sums a row, was a third of the backward pass), whole workgroups through `join` and two barriers.
 template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float* join) {
-#pragma unroll
-    for (int o = (TPR < 64 ? TPR : 64) / 2; o; o >>= 1) v += __shfl_xor(v, o);
+    v = plus_dpp<0xB1>(v);   // lane ^ 1
+    v = plus_dpp<0x4E>(v);   // lane ^ 2
+    v = plus_dpp<0x141>(v);  // the other four of eight
+    if (TPR == 8) return v;
+    v = plus_dpp<0x140>(v);       // the other eight of sixteen
+    v = plus_dpp<0x142, 0xa>(v);  // lane 15 of rows 0 and 2 to rows 1 and 3
+    v = plus_dpp<0x143, 0xc>(v);  // lane 31 to rows 2 and 3: lane 63 has all
+    v = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), 63));
     if (TPR == 256) {
         __syncthreads();
         if ((threadIdx.x & 63) == 0) join[threadIdx.x >> 6] = v;
@@ -61,7 +82,7 @@ __device__ __forceinline__ float row_sum(float v, float* join) {
     return v;
 }
 
-__device__ __forceinline__ float sigmoid(float z) { return 1.f / (1.f + __expf(-z)); }
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
 
 template <class T, int TPR, int NP, bool VEC>
 __global__ __launch_bounds__(kThreads) void norm_forward_kernel(NormArgs a) {
@@ -75,12 +96,21 @@ __global__ __launch_bounds__(kThreads) void norm_forward_kernel(NormArgs a) {
         const long long row = row0 + threadIdx.x / TPR;
         const int width = row < a.rows ? a.width : 0;  // no columns: zeros in, nothing out
         float r[NP][kE], y[NP][kE], sum = 0.f;
+        u32x4 px[NP], pb[NP], pg[NP], pp[NP], pq[NP];  // everything the row needs is asked for first
 #pragma unroll
         for (int i = 0; i < NP; i++) {
             const int c = (i * TPR + t) * kE;
-            load_piece<T, VEC>((const T*)a.x + row * a.x_ld, c, width, r[i]);
+            px[i] = load_piece<T, VEC>((const T*)a.x + row * a.x_ld, c, width);
+            if (a.block) pb[i] = load_piece<T, VEC>((const T*)a.block + row * a.block_ld, c, width);
+            if (a.gate_rows) pg[i] = load_piece<T, VEC>((const T*)a.gate + (a.gate_rows == 2 ? row * a.gate_ld : 0), c, width);
+            if (a.post) pq[i] = load_piece<T, VEC>((const T*)a.post, c, width);
+            if (a.pre) pp[i] = load_piece<T, VEC>((const T*)a.pre, c, width);
+        }
+#pragma unroll
+        for (int i = 0; i < NP; i++) {
+            unpack<T>(px[i], r[i]);
             if (!a.block) continue;
-            load_piece<T, VEC>((const T*)a.block + row * a.block_ld, c, width, y[i]);
+            unpack<T>(pb[i], y[i]);
 #pragma unroll
             for (int e = 0; e < kE; e++) sum += y[i][e] * y[i][e];
         }
@@ -88,15 +118,14 @@ __global__ __launch_bounds__(kThreads) void norm_forward_kernel(NormArgs a) {
             const float inv = 1.f / sqrtf(row_sum<TPR>(sum, join) * inv_width + a.eps);
 #pragma unroll
             for (int i = 0; i < NP; i++) {
-                const int c = (i * TPR + t) * kE;
                 float f[kE];
                 if (a.post) {
-                    load_piece<T, VEC>((const T*)a.post, c, width, f);
+                    unpack<T>(pq[i], f);
 #pragma unroll
                     for (int e = 0; e < kE; e++) y[i][e] *= f[e];
                 }
                 if (a.gate_rows) {
-                    load_piece<T, VEC>((const T*)a.gate + (a.gate_rows == 2 ? row * a.gate_ld : 0), c, width, f);
+                    unpack<T>(pg[i], f);
 #pragma unroll
                     for (int e = 0; e < kE; e++) y[i][e] *= sigmoid(f[e]);
                 }
@@ -118,7 +147,7 @@ __global__ __launch_bounds__(kThreads) void norm_forward_kernel(NormArgs a) {
             const int c = (i * TPR + t) * kE;
             float f[kE];
             if (a.pre) {
-                load_piece<T, VEC>((const T*)a.pre, c, width, f);
+                unpack<T>(pp[i], f);
 #pragma unroll
                 for (int e = 0; e < kE; e++) f[e] *= inv * r[i][e];
             } else {
@@ -157,34 +186,55 @@ __global__ __launch_bounds__(kThreads) void norm_backward_kernel(NormArgs a) {
     const float inv_width = 1.f / (float)a.width;
     const long long step = (long long)gridDim.x * kRows;
     float post_sum[NP][kE] = {}, pre_sum[NP][kE] = {}, gate_sum[NP][kE] = {};
-    for (long long row0 = (long long)blockIdx.x * kRows; row0 < a.rows; row0 += step) {
-        const long long row = row0 + threadIdx.x / TPR;
+    // what every row shares stays in registers; a row's own values are asked for while the row before it is worked on
+    u32x4 w_post[NP], w_pre[NP], w_gate[NP], x_[NP], block_[NP], gate_[NP], dr_[NP], dh_[NP];
+#pragma unroll
+    for (int i = 0; i < NP; i++) {
+        const int c = (i * TPR + t) * kE;
+        if (a.post) w_post[i] = load_piece<T, VEC>((const T*)a.post, c, a.width);
+        if (a.pre) w_pre[i] = load_piece<T, VEC>((const T*)a.pre, c, a.width);
+        if (a.gate_rows == 1) w_gate[i] = load_piece<T, VEC>((const T*)a.gate, c, a.width);
+        dr_[i] = dh_[i] = u32x4{0, 0, 0, 0};
+    }
+    auto ask = [&](long long row) {
         const int width = row < a.rows ? a.width : 0;
-        float r[NP][kE], nb[NP][kE], s[NP][kE], dh[NP][kE], f[kE], sum = 0.f;
 #pragma unroll
         for (int i = 0; i < NP; i++) {
             const int c = (i * TPR + t) * kE;
-            load_piece<T, VEC>((const T*)a.x + row * a.x_ld, c, width, r[i]);
-            if (a.dh) load_piece<T, VEC>((const T*)a.dh + row * a.width, c, width, dh[i]);
-            else
+            x_[i] = load_piece<T, VEC>((const T*)a.x + row * a.x_ld, c, width);
+            if (a.block) block_[i] = load_piece<T, VEC>((const T*)a.block + row * a.block_ld, c, width);
+            if (a.gate_rows == 2) gate_[i] = load_piece<T, VEC>((const T*)a.gate + row * a.gate_ld, c, width);
+            if (a.dh) dh_[i] = load_piece<T, VEC>((const T*)a.dh + row * a.width, c, width);
+            if (a.dr) dr_[i] = load_piece<T, VEC>((const T*)a.dr + row * a.width, c, width);
+        }
+    };
+    const long long first = (long long)blockIdx.x * kRows;
+    if (first < a.rows) ask(first + threadIdx.x / TPR);
+    for (long long row0 = first; row0 < a.rows; row0 += step) {
+        const long long row = row0 + threadIdx.x / TPR;
+        const int width = row < a.rows ? a.width : 0;
+        float r[NP][kE], nb[NP][kE], s[NP][kE], dh[NP][kE], d_[NP][kE], f[kE], sum = 0.f;
 #pragma unroll
-                for (int e = 0; e < kE; e++) dh[i][e] = 0.f;
+        for (int i = 0; i < NP; i++) {
+            unpack<T>(x_[i], r[i]);
+            unpack<T>(dh_[i], dh[i]);
+            unpack<T>(dr_[i], d_[i]);
             if (!a.block) continue;
-            load_piece<T, VEC>((const T*)a.block + row * a.block_ld, c, width, nb[i]);
-            if (a.gate_rows) load_piece<T, VEC>((const T*)a.gate + (a.gate_rows == 2 ? row * a.gate_ld : 0), c, width, s[i]);
+            unpack<T>(block_[i], nb[i]);
+            if (a.gate_rows) unpack<T>(a.gate_rows == 2 ? gate_[i] : w_gate[i], s[i]);
 #pragma unroll
             for (int e = 0; e < kE; e++) {
                 sum += nb[i][e] * nb[i][e];
                 s[i][e] = a.gate_rows ? sigmoid(s[i][e]) : 1.f;
             }
         }
+        if (row0 + step < a.rows) ask(row + step);
         float inv_b = 0.f;
         if (a.block) {
             inv_b = 1.f / sqrtf(row_sum<TPR>(sum, join) * inv_width + a.eps);
 #pragma unroll
             for (int i = 0; i < NP; i++) {
-                const int c = (i * TPR + t) * kE;
-                if (a.post) load_piece<T, VEC>((const T*)a.post, c, width, f);
+                if (a.post) unpack<T>(w_post[i], f);
 #pragma unroll
                 for (int e = 0; e < kE; e++) {
                     nb[i][e] *= inv_b;
@@ -195,7 +245,7 @@ __global__ __launch_bounds__(kThreads) void norm_backward_kernel(NormArgs a) {
         float rr = 0.f, gr = 0.f;
 #pragma unroll
         for (int i = 0; i < NP; i++) {
-            if (a.pre) load_piece<T, VEC>((const T*)a.pre, (i * TPR + t) * kE, width, f);
+            if (a.pre) unpack<T>(w_pre[i], f);
 #pragma unroll
             for (int e = 0; e < kE; e++) {
                 rr += r[i][e] * r[i][e];
@@ -209,17 +259,13 @@ __global__ __launch_bounds__(kThreads) void norm_backward_kernel(NormArgs a) {
         for (int i = 0; i < NP; i++) {
             const int c = (i * TPR + t) * kE;
             float d[kE], fp[kE], fq[kE];
-            if (a.dr) load_piece<T, VEC>((const T*)a.dr + row * a.width, c, width, d);
-            else
-#pragma unroll
-                for (int e = 0; e < kE; e++) d[e] = 0.f;
-            if (a.pre) load_piece<T, VEC>((const T*)a.pre, c, width, fp);
-            if (a.post) load_piece<T, VEC>((const T*)a.post, c, width, fq);
+            if (a.pre) unpack<T>(w_pre[i], fp);
+            if (a.post) unpack<T>(w_post[i], fq);
 #pragma unroll
             for (int e = 0; e < kE; e++) {
                 const float n = r[i][e] * inv_r;
                 pre_sum[i][e] += dh[i][e] * n;
-                d[e] += inv_r * (dh[i][e] * (a.pre ? fp[e] : 1.f) - n * mean_gr);
+                d[e] = d_[i][e] + inv_r * (dh[i][e] * (a.pre ? fp[e] : 1.f) - n * mean_gr);
                 r[i][e] = d[e];  // t
             }
             if (a.dx) store_piece<T, VEC>((T*)a.dx + row * a.width, c, width, d);
@@ -252,21 +298,23 @@ __global__ __launch_bounds__(kThreads) void norm_backward_kernel(NormArgs a) {
     if (a.dgate && a.gate_rows == 1) column_sum<TPR, NP, kE>(gate_sum, out + 2 * a.width, a.width, buf);
 }
 
-// Joins the workgroups' column sums in a fixed order: 32 columns a workgroup, eight threads a column.
+// Joins the workgroups' column sums in a fixed order: 32 columns a workgroup, 32 threads a column.
 template <class T>
-__global__ __launch_bounds__(kThreads) void norm_join_kernel(const float* work, T* dpost, T* dpre, T* dgate, int width, int parts) {
-    __shared__ float join[8][32];
+__global__ __launch_bounds__(kJoinThreads) void norm_join_kernel(const float* work, T* dpost, T* dpre, T* dgate, int width, int parts) {
+    constexpr int kSlices = kJoinThreads / 32;
+    __shared__ float join[kSlices][32];
     const int which = blockIdx.y, c = blockIdx.x * 32 + (threadIdx.x & 31), k0 = threadIdx.x >> 5;
     T* out = which == 0 ? dpost : which == 1 ? dpre : dgate;
     if (!out) return;
     float s = 0.f;
     if (c < width)
-        for (int k = k0; k < parts; k += 8) s += work[((long long)k * 3 + which) * width + c];
+#pragma unroll 8
+        for (int k = k0; k < parts; k += kSlices) s += work[((long long)k * 3 + which) * width + c];
     join[k0][threadIdx.x & 31] = s;
     __syncthreads();
     if (k0 || c >= width) return;
 #pragma unroll
-    for (int k = 1; k < 8; k++) s += join[k][threadIdx.x];
+    for (int k = 1; k < kSlices; k++) s += join[k][threadIdx.x];
     out[c] = (T)s;
 }
 
@@ -291,7 +339,7 @@ int run(const NormArgs& a, bool backward, hipStream_t s) {
     int rc = (int)hipGetLastError();
     T* dgate = a.gate_rows == 1 ? (T*)a.dgate : nullptr;
     if (rc || !(a.dpost || a.dpre || dgate)) return rc;
-    norm_join_kernel<T><<<dim3((a.width + 31) / 32, 3), kThreads, 0, s>>>(a.work, (T*)a.dpost, (T*)a.dpre, dgate, a.width, blocks);
+    norm_join_kernel<T><<<dim3((a.width + 31) / 32, 3), kJoinThreads, 0, s>>>(a.work, (T*)a.dpost, (T*)a.dpre, dgate, a.width, blocks);
     return (int)hipGetLastError();
 }
 
