@@ -249,14 +249,14 @@ struct TransTile {
 
 // D += A B^T over one pair of 16-byte pieces per lane (the lane's half of the wave picks the piece, so a step spans 32 B of
 // the reduction axis). The order of the reduction inside a step is the same for both operands, which is all the product needs.
-__device__ __forceinline__ void mfma(f32x16& d, const u32x4& a, const u32x4& b, float) {
+[[maybe_unused]] __device__ __forceinline__ void mfma(f32x16& d, const u32x4& a, const u32x4& b, float) {
 #pragma unroll
     for (int e = 0; e < 4; e++) d = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[e]), __uint_as_float(b[e]), d, 0, 0, 0);
 }
-__device__ __forceinline__ void mfma(f32x16& d, const u32x4& a, const u32x4& b, __bf16) {
+[[maybe_unused]] __device__ __forceinline__ void mfma(f32x16& d, const u32x4& a, const u32x4& b, __bf16) {
     d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), d, 0, 0, 0);
 }
-__device__ __forceinline__ void mfma(f32x16& d, const u32x4& a, const u32x4& b, _Float16) {
+[[maybe_unused]] __device__ __forceinline__ void mfma(f32x16& d, const u32x4& a, const u32x4& b, _Float16) {
     d = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), d, 0, 0, 0);
 }
 
@@ -377,7 +377,7 @@ __device__ __forceinline__ void write_results(const LinearArgs& a, const f32x16 
 
 // BM x BN outputs a workgroup (rows x features), WM x WN waves.
 template <class T, Product P, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * 64, 2) void linear_kernel(LinearArgs a, int tiles_n, long long tiles, int parts, long long red_part) {
+__global__ __launch_bounds__(WM * WN * 64, 2) void linear_kernel(LinearArgs a, float* db_work, int tiles_n, long long tiles, int parts, long long red_part) {
     using Slope = typename Elem<T>::Slope;
     constexpr int kThreads = WM * WN * 64, kE = Elem<T>::kE, kK = kPieces * kE, TM = BM / WM / 32, TN = BN / WN / 32;
     static_assert(TM >= 1 && TN >= 1 && BM % (kThreads / 8) == 0 && BN % (kThreads / 8) == 0, "a whole number of pieces for each thread");
@@ -461,7 +461,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void linear_kernel(LinearArgs a, i
                 float s = 0.f;
 #pragma unroll
                 for (int c = 0; c < kPieces; c++) s += join[c * BM + i];
-                a.work[(long long)parts * a.out * a.in + unit.part * a.out + row0 + i] = s;
+                db_work[unit.part * a.out + row0 + i] = s;
             }
         }
     }
@@ -557,6 +557,9 @@ struct StreamTile {
     }
 };
 
+// Elements of a row of n with its last piece made whole (padded rows hold zeros there).
+template <class T> __host__ __device__ __forceinline__ long long whole_pieces(long long n) { return (n + Elem<T>::kE - 1) / Elem<T>::kE * Elem<T>::kE; }
+
 // Waits until at most LEFT of the wave's loads are under way (its LDS accesses all done), then for the workgroup.
 template <int LEFT>
 __device__ __forceinline__ void landed() {
@@ -584,13 +587,13 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void linear_stream_kernel(LinearAr
     } else if (P == kInput) {
         nrows = a.rows; nfeat = a.in; red1 = a.out;
         rt.init((const T*)a.dy, a.dy_ld, row0, nrows);
-        ft.init((const T*)a.w, a.w_ld, feat0, nfeat);
+        ft.init((const T*)a.w, a.w_ld, feat0, whole_pieces<T>(nfeat));
     } else {
         nrows = a.out; nfeat = a.in;
         red0 = unit.part * red_part;
         red1 = red0 + red_part < a.rows ? red0 + red_part : a.rows;
-        rt.init((const T*)a.dy, a.dy_ld, row0, nrows);
-        ft.init((const T*)a.x, a.x_ld, feat0, nfeat);
+        rt.init((const T*)a.dy, a.dy_ld, row0, whole_pieces<T>(nrows));
+        ft.init((const T*)a.x, a.x_ld, feat0, whole_pieces<T>(nfeat));
     }
     auto stage = [&](int to, long long k) {
         if (k + kK <= red1) {
@@ -778,11 +781,11 @@ __global__ __launch_bounds__(kResidentWaves * 64, 2 * PER_CU) void linear_reside
     }
 }
 
-// dz = dy * slope, rounded once to T, into a dense [rows][out] buffer (or nowhere: dz is dy), and the bias gradient's partial
+// dz = dy * slope, rounded once to T, into rows of whole pieces (or nowhere: dz is dy), and the bias gradient's partial
 // sums of the 32-bit values: thread (c, g) of a workgroup owns piece c of a strip of kStrip pieces and every kGroups-th of the
 // workgroup's rows.
 template <class T>
-__global__ __launch_bounds__(256) void linear_dz_kernel(LinearArgs a, T* dz, float* partial, long long rows_part) {
+__global__ __launch_bounds__(256) void linear_dz_kernel(LinearArgs a, T* dz, long long dz_ld, float* partial, long long rows_part) {
     using Slope = typename Elem<T>::Slope;
     constexpr int kE = Elem<T>::kE, kStrip = 32, kGroups = 8;
     __shared__ float join[kGroups][kStrip * kE];
@@ -793,16 +796,17 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(LinearArgs a, T* dz, flo
     if (left > 0)
 #pragma unroll 4
         for (long long r = row0 + g; r < row1; r += kGroups) {
-            const auto v = load_n<T, kE>((const T*)a.dy + r * a.dy_ld + col, kE);
+            const bool whole = a.out % kE == 0;  // the same for the launch
+            const auto v = whole ? load_n<T, kE>((const T*)a.dy + r * a.dy_ld + col, kE) : load_end<T, kE>((const T*)a.dy + r * a.dy_ld, col, a.out);
             float f[kE];
 #pragma unroll
             for (int e = 0; e < kE; e++) f[e] = to_f(v.e[e]);
             if (a.slope) {
-                const auto q = load_n<Slope, kE>((const Slope*)a.slope + r * a.out + col, kE);
+                const auto q = whole ? load_n<Slope, kE>((const Slope*)a.slope + r * a.out + col, kE) : load_end<Slope, kE>((const Slope*)a.slope + r * a.out, col, a.out);
 #pragma unroll
                 for (int e = 0; e < kE; e++) f[e] *= to_f(q.e[e]);
             }
-            if (dz) store_n<T, kE>(dz + r * a.out + col, kE, f);
+            if (dz) store_n<T, kE>(dz + r * dz_ld + col, kE, f);
 #pragma unroll
             for (int e = 0; e < kE; e++) sum[e] += f[e];
         }
@@ -816,6 +820,253 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(LinearArgs a, T* dz, flo
 #pragma unroll
         for (int k = 0; k < kGroups; k++) s += join[k][i];
         partial[(long long)blockIdx.x * a.out + first + i] = s;
+    }
+}
+
+// Rows of `cols` elements into rows of whole, aligned pieces, zeros behind their end.
+template <class T>
+__global__ __launch_bounds__(256) void linear_pad_kernel(const T* from, long long ld, long long rows, int cols, T* to, int pieces) {
+    constexpr int kE = Elem<T>::kE;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < rows * pieces; i += (long long)gridDim.x * 256) {
+        const long long r = i / pieces;
+        const int p = (int)(i - r * pieces);
+        *(u32x4*)(to + (r * pieces + p) * kE) = __builtin_bit_cast(u32x4, load_end<T, kE>(from + r * ld, p * kE, cols));
+    }
+}
+
+// ---- the whole gradient of a narrow layer (up to 128 x 128, 256 x 64) in one pass: dy, the slopes and x are read
+// once, dx is written once, the weight gradient stays in the accumulators of persistent workgroups until their last tile.
+// A tile of rows arrives in LDS, is turned into dz there (each thread its own pieces, adding up the bias gradient), and is
+// then the row operand of dx (weights in registers) and, read transposed, of the weight gradient. ----
+constexpr int kBackThreads = 512, kBackWaves = 8;
+
+// Piece p of row r at p ^ back_swz(r): sixteen rows' same piece in different banks (dx), and four neighbouring rows' 64-byte
+// blocks too (the transposed reads).
+template <int PIECES> __device__ __forceinline__ int back_swz(int r) {
+    return PIECES >= 16 ? ((r & 3) << 2) | ((r >> 2) & 3) : PIECES == 8 ? ((r >> 1) & 1) << 2 | ((r >> 2) & 3) : (r >> 2) & 3;
+}
+
+// A [ROWS][PIECES] tile of LDS filled by eight waves; the same number of loads for every wave.
+template <class E, int ROWS, int PIECES>
+struct BackTile {
+    static constexpr int kE = 16 / sizeof(E), kCount = ROWS * PIECES, kLoads = kCount / 64, kN = (kLoads + kBackWaves - 1) / kBackWaves;
+    __device__ __forceinline__ static int at(int r, int piece) { return r * PIECES + (piece ^ back_swz<PIECES>(r)); }
+    __device__ __forceinline__ static int load_of(int i) { return ((threadIdx.x >> 6) + i * kBackWaves) % kLoads; }
+    __device__ __forceinline__ static int slot(int i) { return load_of(i) * 64 + (threadIdx.x & 63); }
+    __device__ __forceinline__ static int row_of(int s) { return s / PIECES; }
+    __device__ __forceinline__ static int piece_of(int s) { return (s % PIECES) ^ back_swz<PIECES>(s / PIECES); }
+    __device__ __forceinline__ static void clear(u32x4* lds, int pieces) {
+        for (int s = threadIdx.x; s < kCount; s += kBackThreads) if (piece_of(s) >= pieces) lds[s] = u32x4{0, 0, 0, 0};
+    }
+    __device__ __forceinline__ static void stage(u32x4* lds, const E* p, long long ld, long long row0, long long rows, int pieces) {
+#pragma unroll
+        for (int i = 0; i < kN; i++) {
+            const int s = slot(i), piece = piece_of(s);
+            const long long r0 = row0 + row_of(s), r = r0 < rows ? r0 : rows - 1;
+            if (piece < pieces)  // (64 slots hold a whole row or more: some lane of every load takes part)
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(p + r * ld + piece * kE),
+                                                 (__attribute__((address_space(3))) void*)(lds + load_of(i) * 64), 16, 0, 0);
+        }
+    }
+    // Fragment of columns block ... block + 31 (as `features` of the product or as its rows) over the reduction step s of rows.
+    template <bool FEATURES>
+    __device__ __forceinline__ static u32x4 transposed(const u32x4* lds, int block, int row0) {
+        const int lane = threadIdx.x & 63, half = lane >> 5;
+        if constexpr (sizeof(E) == 2) {
+            const int i = (lane & 16) + 4 * (lane & 3), f = block + (FEATURES ? feature_of<E>(i) : i), m0 = (lane & 15) >> 2;
+            union { u32x4 u; s16x4 h[2]; } v;
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const int m = row0 + 8 * half + 4 * t + m0;
+                v.h[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)((const char*)(lds + at(m, f / kE)) + f % kE * 2));
+            }
+            return v.u;
+        } else {
+            const int f = block + (lane & 31);
+            u32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = ((const uint32_t*)(lds + at(row0 + 4 * half + e, f / kE)))[f % kE];
+            return v;
+        }
+    }
+};
+
+template <class T, int OB, int IB>
+struct Back {
+    using Slope = typename Elem<T>::Slope;
+    static constexpr int kE = Elem<T>::kE, kPo = OB * 32 / kE, kPi = IB * 32 / kE, kPs = OB * 32 / (16 / (int)sizeof(Slope));
+    static constexpr int kRowBytes = (kPo + kPi + kPs) * 16;
+    // rows of a tile: three tiles in LDS, at most 32 for each of the waves that share a feature block
+    static constexpr int kMost = 32 * (kBackWaves / IB), kFit = 152 * 1024 / 3 / kRowBytes, kRows = kFit >= kMost ? kMost : kFit >= 128 ? (kMost < 128 ? kMost : 128) : kFit >= 64 ? (kMost < 64 ? kMost : 64) : 32;
+    static constexpr int kTile = kRows * (kPo + kPi + kPs), kStages = 152 * 1024 / (kTile * 16) > 6 ? 6 : 152 * 1024 / (kTile * 16);
+    static_assert(kStages >= 2 && kRows >= 32, "at least one tile ahead");
+    using Dy = BackTile<T, kRows, kPo>;
+    using X = BackTile<T, kRows, kPi>;
+    using S = BackTile<Slope, kRows, kPs>;
+    static constexpr int kS = kRows * kPo, kX = kS + kRows * kPs;  // offsets in a tile: dy, slopes, x
+    static constexpr int kBlocks = OB * IB, kMine = kBlocks > kBackWaves ? kBlocks / kBackWaves : 1;      // 32 x 32 blocks of the weight gradient, a wave's
+    static constexpr int kSlices = kBlocks < kBackWaves ? kBackWaves / kBlocks : 1;                       // waves that share a block, each its rows
+    static constexpr int kStep = 32 / (int)sizeof(T);                                                     // rows of a reduction step
+    static constexpr int kSliceRows = kRows / kSlices >= kStep ? kRows / kSlices : kStep;
+    static constexpr int kDxTurns = kRows / 32 * IB / kBackWaves > 0 ? kRows / 32 * IB / kBackWaves : 1;  // a wave's 32 x 32 blocks of dx
+    static constexpr int kSteps = kPo / 2;                                                                // reduction steps of dx
+};
+
+template <class T, int OB, int IB>
+__global__ __launch_bounds__(kBackThreads, 2) void linear_back_kernel(LinearArgs a, float* db_work, int blocks) {
+    using M = Back<T, OB, IB>;
+    using Slope = typename M::Slope;
+    constexpr int kE = M::kE, kQ = 16 / kE, kRows = M::kRows, kStages = M::kStages, kPieces2 = (kRows * M::kPo + kBackThreads - 1) / kBackThreads;
+    using Piece = Vec<T, kE>;
+    using SlopePiece = Vec<Slope, 16 / sizeof(Slope)>;
+    __shared__ u32x4 lds[kStages][M::kTile];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l32 = lane & 31;
+    const int tiles = (int)((a.rows + kRows - 1) / kRows);
+    int tile = blockIdx.x;
+    const int po = (a.out + kE - 1) / kE, pi = (a.in + kE - 1) / kE, ps = a.out / (16 / (int)sizeof(Slope));
+    const bool slopes = a.slope != nullptr;
+    auto stage = [&](int to, int t) {
+        const long long row0 = (long long)t * kRows;
+        M::Dy::stage(lds[to], (const T*)a.dy, a.dy_ld, row0, a.rows, po);
+        if (slopes) M::S::stage(lds[to] + M::kS, (const Slope*)a.slope, a.out, row0, a.rows, ps);
+        M::X::stage(lds[to] + M::kX, (const T*)a.x, a.x_ld, row0, a.rows, pi);
+    };
+#pragma unroll
+    for (int i = 0; i < kStages; i++) {
+        M::Dy::clear(lds[i], po);
+        M::S::clear(lds[i] + M::kS, ps);
+        M::X::clear(lds[i] + M::kX, pi);
+    }
+    // dx: feature block wave % IB, the weights' column fragments
+    const int fb = wave % IB * 32, rg = wave / IB;
+    u32x4 w[M::kSteps];
+    if (a.dx) {
+        const int f = fb + feature_of<T>(l32);
+#pragma unroll
+        for (int s = 0; s < M::kSteps; s++) {
+            Vec<T, kE> v;
+#pragma unroll
+            for (int e = 0; e < kE; e++) {
+                const int n = (2 * s + half) * kE + e;
+                v.e[e] = f < a.in && n < a.out ? ((const T*)a.w)[(long long)n * a.w_ld + f] : (T)0.f;
+            }
+            w[s] = __builtin_bit_cast(u32x4, v);
+        }
+    }
+    // weight gradient: column block ib, row blocks ob + j kBackWaves / IB, rows slice ... of a tile
+    const int ib = wave % IB * 32, slice = M::kSlices > 1 ? wave / M::kBlocks : 0, ob = M::kSlices > 1 ? (wave % M::kBlocks) / IB : wave / IB;
+    f32x16 dw[M::kMine] = {};
+    float sum[kPieces2][kE] = {};
+#pragma unroll
+    for (int i = 0; i < kStages - 1; i++)
+        if (tile + i * blocks < tiles) stage(i, tile + i * blocks);
+    int buf = 0;
+    for (; tile < tiles; tile += blocks) {
+        // this tile has landed when only the loads of the kStages - 2 behind it are left (without slopes there are fewer)
+        constexpr int kFew = (kStages - 2) * (M::Dy::kN + M::X::kN), kAll = kFew + (kStages - 2) * M::S::kN;
+        if (tile + (kStages - 2) * blocks >= tiles) landed<0>();
+        else if (slopes) landed<kAll>();
+        else landed<kFew>();
+        const int next = buf == 0 ? kStages - 1 : buf - 1;
+        if (tile + (kStages - 1) * blocks < tiles) stage(next, tile + (kStages - 1) * blocks);
+        u32x4* t = lds[buf];
+        const long long row0 = (long long)tile * kRows;
+        const bool last = row0 + kRows > a.rows;
+#pragma unroll
+        for (int i = 0; i < kPieces2; i++) {  // dy -> dz in place
+            const int s = threadIdx.x + i * kBackThreads;
+            if (kRows * M::kPo % kBackThreads && s >= kRows * M::kPo) break;
+            const int r = M::Dy::row_of(s), piece = M::Dy::piece_of(s);
+            auto v = __builtin_bit_cast(Piece, t[s]);
+            float f[kE];
+#pragma unroll
+            for (int e = 0; e < kE; e++) f[e] = to_f(v.e[e]);
+            if (slopes) {
+                constexpr int kPer = sizeof(Slope) * kE / 16, kSE = 16 / sizeof(Slope);
+#pragma unroll
+                for (int k = 0; k < kPer; k++) {
+                    const auto q = __builtin_bit_cast(SlopePiece, t[M::kS + M::S::at(r, piece * kPer + k)]);
+#pragma unroll
+                    for (int e = 0; e < kSE; e++) f[k * kSE + e] *= to_f(q.e[e]);
+                }
+            }
+            if (last && row0 + r >= a.rows)
+#pragma unroll
+                for (int e = 0; e < kE; e++) f[e] = 0.f;
+#pragma unroll
+            for (int e = 0; e < kE; e++) sum[i][e] += f[e];
+            if (slopes || last) {
+#pragma unroll
+                for (int e = 0; e < kE; e++) v.e[e] = (T)f[e];
+                t[s] = __builtin_bit_cast(u32x4, v);
+            }
+        }
+        if (last)  // rows past the end repeat the last one: no x of theirs, be it an infinity, meets a zero dz
+            for (int s = threadIdx.x; s < M::X::kCount; s += kBackThreads) if (row0 + M::X::row_of(s) >= a.rows) t[M::kX + s] = u32x4{0, 0, 0, 0};
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (a.dx) {
+#pragma unroll
+            for (int i = 0; i < M::kDxTurns; i++) {
+                const int r0 = (rg + i * (kBackWaves / IB)) * 32;
+                if (r0 >= kRows) break;
+                f32x16 acc = {};
+#pragma unroll
+                for (int s = 0; s < M::kSteps; s++) mfma(acc, w[s], t[M::Dy::at(r0 + l32, 2 * s + half)], T{});
+                const long long row = row0 + r0 + l32;
+                if (row < a.rows)
+#pragma unroll
+                    for (int q = 0; q < kQ; q++) {
+                        const int feat = fb + piece_feature<T>(q, half);
+                        if (feat >= a.in) continue;
+                        float v[kE];
+#pragma unroll
+                        for (int j = 0; j < kE; j++) v[j] = acc[q * kE + j];
+                        store_n<T, kE>((T*)a.dx + row * a.dx_ld + feat, a.in - feat, v);
+                    }
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < M::kSliceRows / M::kStep; s++) {
+            const int m = slice * M::kSliceRows + s * M::kStep;
+            if (M::kSlices * M::kSliceRows > kRows && m >= kRows) break;
+            const u32x4 ff = M::X::template transposed<true>(t + M::kX, ib, m);
+#pragma unroll
+            for (int j = 0; j < M::kMine; j++) mfma(dw[j], ff, M::Dy::template transposed<false>(t, (ob + j * (kBackWaves / IB)) * 32, m), T{});
+        }
+        buf = buf == kStages - 1 ? 0 : buf + 1;
+    }
+    const long long part = (long long)blockIdx.x * M::kSlices + slice, weights = (long long)a.out * a.in;
+#pragma unroll
+    for (int j = 0; j < M::kMine; j++) {
+        const int n = (ob + j * (kBackWaves / IB)) * 32 + l32;
+        if (n >= a.out) continue;
+#pragma unroll
+        for (int q = 0; q < kQ; q++) {
+            const int feat = ib + piece_feature<T>(q, half);
+            if (feat >= a.in) continue;
+            float v[kE];
+#pragma unroll
+            for (int e = 0; e < kE; e++) v[e] = dw[j][q * kE + e];
+            store_n<float, kE>(a.work + part * weights + (long long)n * a.in + feat, a.in - feat, v);
+        }
+    }
+    if (!a.db) return;
+    __syncthreads();
+    float* join = (float*)lds;
+#pragma unroll
+    for (int i = 0; i < kPieces2; i++) {
+        const int s = threadIdx.x + i * kBackThreads;
+        if (s < kRows * M::kPo)
+#pragma unroll
+            for (int e = 0; e < kE; e++) join[s * kE + e] = sum[i][e];
+    }
+    __syncthreads();
+    for (int n = threadIdx.x; n < a.out; n += kBackThreads) {
+        float s = 0.f;
+        for (int r = 0; r < kRows; r++) s += join[M::Dy::at(r, n / kE) * kE + n % kE];
+        db_work[(long long)blockIdx.x * a.out + n] = s;
     }
 }
 
@@ -843,10 +1094,10 @@ __global__ __launch_bounds__(kJoinThreads) void linear_join_kernel(const float* 
 }
 
 template <class T, Product P, int BM, int BN, int WM, int WN>
-int launch(const LinearArgs& a, long long nrows, long long nfeat, int parts, long long red_part, hipStream_t s) {
+int launch(const LinearArgs& a, long long nrows, long long nfeat, int parts, long long red_part, hipStream_t s, float* db_work = nullptr) {
     const int tiles_n = (int)((nfeat + BN - 1) / BN);
     const long long tiles = (nrows + BM - 1) / BM * tiles_n, units = tiles * parts;
-    linear_kernel<T, P, BM, BN, WM, WN><<<(unsigned)((units + 7) / 8 * 8), WM * WN * 64, 0, s>>>(a, tiles_n, tiles, parts, red_part);
+    linear_kernel<T, P, BM, BN, WM, WN><<<(unsigned)((units + 7) / 8 * 8), WM * WN * 64, 0, s>>>(a, db_work, tiles_n, tiles, parts, red_part);
     return (int)hipGetLastError();
 }
 
@@ -878,13 +1129,13 @@ Split split_of(long long rows, int in, int out) {
 }
 
 template <class T>
-int weight_grad(const LinearArgs& a, const Split& sp, hipStream_t s) {
+int weight_grad(const LinearArgs& a, float* db_work, const Split& sp, hipStream_t s) {
     constexpr int kK = kPieces * Elem<T>::kE;
     const long long part = ((a.rows + sp.parts - 1) / sp.parts + kK - 1) / kK * kK;
-    if (sp.bm == 64 && sp.bn == 64) return launch<T, kWeight, 64, 64, 2, 2>(a, a.out, a.in, sp.parts, part, s);
-    if (sp.bm == 64) return launch<T, kWeight, 64, 128, 2, 2>(a, a.out, a.in, sp.parts, part, s);
-    if (sp.bn == 64) return launch<T, kWeight, 128, 64, 2, 2>(a, a.out, a.in, sp.parts, part, s);
-    return launch<T, kWeight, 128, 128, 2, 2>(a, a.out, a.in, sp.parts, part, s);
+    if (sp.bm == 64 && sp.bn == 64) return launch<T, kWeight, 64, 64, 2, 2>(a, a.out, a.in, sp.parts, part, s, db_work);
+    if (sp.bm == 64) return launch<T, kWeight, 64, 128, 2, 2>(a, a.out, a.in, sp.parts, part, s, db_work);
+    if (sp.bn == 64) return launch<T, kWeight, 128, 64, 2, 2>(a, a.out, a.in, sp.parts, part, s, db_work);
+    return launch<T, kWeight, 128, 128, 2, 2>(a, a.out, a.in, sp.parts, part, s, db_work);
 }
 
 template <class T, Product P, int BM, int BN, int WM, int WN, int PIECES, int STAGES>
@@ -904,40 +1155,6 @@ int stream_product(const LinearArgs& a, long long feats, hipStream_t s) {
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 constexpr int kDzParts = 512;
-
-// Whether the backward pass forms dz in a pass of its own and streams both products.
-template <class T>
-bool streams_backward(const LinearArgs& a) {
-    constexpr int kE = Elem<T>::kE;
-    return a.in % kE == 0 && a.out % kE == 0 && a.w_ld % kE == 0 && a.dy_ld % kE == 0 && a.x_ld % kE == 0 && aligned16(a.w) && aligned16(a.dy) && aligned16(a.x) && aligned16(a.slope) &&
-           a.in > 64 && a.out > 64 && !few(a.rows, a.in);
-}
-
-template <class T>
-int backward_stream(LinearArgs a, hipStream_t s) {
-    constexpr int kE = Elem<T>::kE, kK = kPieces * kE;
-    const Split sp = split_of(a.rows, a.in, a.out);
-    const long long weights = (long long)a.out * a.in;
-    float* db_work = a.work + sp.parts * weights;
-    T* dz = (T*)(db_work + ((long long)kDzParts * a.out + 3) / 4 * 4);
-    const long long rows_part = (a.rows + kDzParts - 1) / kDzParts;
-    const int dz_parts = (int)((a.rows + rows_part - 1) / rows_part);
-    int rc = 0;
-    if (a.slope || a.db) {
-        linear_dz_kernel<T><<<dim3(dz_parts, (a.out + 32 * kE - 1) / (32 * kE)), 256, 0, s>>>(a, a.slope && (a.dx || a.dw) ? dz : nullptr, a.db ? db_work : nullptr, rows_part);
-        if ((rc = (int)hipGetLastError())) return rc;
-    }
-    if (a.slope) { a.dy = dz; a.dy_ld = a.out; }
-    if (a.dx && (rc = stream_product<T, kInput>(a, a.in, s))) return rc;
-    if (a.dw) {
-        const long long part = ((a.rows + sp.parts - 1) / sp.parts + kK - 1) / kK * kK;
-        if ((rc = stream<T, kWeight, 128, 128, 2, 2, 8, 2>(a, a.out, a.in, sp.parts, part, s))) return rc;
-    }
-    if (!a.dw && !a.db) return 0;
-    const long long all = (a.dw ? weights : 0) + (a.db ? a.out : 0);
-    linear_join_kernel<T><<<(unsigned)((all + 31) / 32), kJoinThreads, 0, s>>>(a.work, db_work, (T*)a.dw, (T*)a.db, weights, a.out, sp.parts, dz_parts);
-    return (int)hipGetLastError();
-}
 
 // Persistent workgroups: as many as stay on the card at once, in whole multiples of the feature groups for each XCD.
 template <class T, int KS, int WF, bool RES>
@@ -994,35 +1211,152 @@ int forward_any(const LinearArgs& a, hipStream_t s) {
     return product<T, kForward>(a, a.out, s);
 }
 
+// The class of a width in blocks of 32: 2, 4, 8 (f32: up to 4), 0 where the one-pass gradient does not reach. Wider pairs than
+// 16 blocks spill (131072 x 256 x 256 bf16 in one pass: 240 us; in three: 190).
 template <class T>
-int backward_any(const LinearArgs& a, hipStream_t s) {
-    if (streams_backward<T>(a)) return backward_stream<T>(a, s);
-    int rc = 0;
-    if (a.dx && a.rows && (rc = product<T, kInput>(a, a.in, s))) return rc;
-    if (a.dw || a.db) {
-        const Split sp = split_of(a.rows, a.in, a.out);
-        if ((rc = weight_grad<T>(a, sp, s))) return rc;
-        const long long weights = (long long)a.out * a.in, all = (a.dw ? weights : 0) + (a.db ? a.out : 0);
-        linear_join_kernel<T><<<(unsigned)((all + 31) / 32), kJoinThreads, 0, s>>>(a.work, a.work + sp.parts * weights, (T*)a.dw, (T*)a.db, weights, a.out, sp.parts, sp.parts);
-        rc = (int)hipGetLastError();
+int blocks_of(int n) { return n <= 64 ? 2 : n <= 128 ? 4 : n <= 256 && sizeof(T) == 2 ? 8 : 0; }
+
+// f(OB, IB) as types, for the classes of out and in; false if there is none.
+template <class T, class F>
+bool visit_back(int out, int in, F f) {
+    const int ob = blocks_of<T>(out), ib = blocks_of<T>(in);
+    if (!ob || !ib || ob * ib > 16) return false;
+    using Two = std::integral_constant<int, 2>;
+    using Four = std::integral_constant<int, 4>;
+    using Eight = std::integral_constant<int, 8>;
+    if (ob == 2 && ib == 2) f(Two{}, Two{});
+    else if (ob == 2 && ib == 4) f(Two{}, Four{});
+    else if (ob == 4 && ib == 2) f(Four{}, Two{});
+    else if (ob == 4 && ib == 4) f(Four{}, Four{});
+    else if constexpr (sizeof(T) == 2) {
+        if (ob == 2) f(Two{}, Eight{}); else f(Eight{}, Two{});
     }
-    return rc;
+    return true;
+}
+
+// Workgroups: one a CU, each with enough tiles that its partial sum of the weight gradient is not most of what it moves.
+template <class M>
+int back_blocks(long long rows, int in, int out) {
+    const long long tiles = (rows + M::kRows - 1) / M::kRows, least = (long long)in * out >= 128 * 128 ? 4 : 1, b = (tiles + least - 1) / least;
+    return b < 1 ? 1 : b > 256 ? 256 : (int)b;
+}
+
+// How a gradient is computed: one plan for the workspace's size and the launches. Pieces: rows of x and dy (and w) are whole,
+// aligned 16-byte pieces, as they are or after dz and copies of x and w have been laid out so.
+struct Plan {
+    bool narrow, stream, pad;
+    size_t dw, db, dz, x, w, bytes;  // offsets into the workspace: partial sums, then the laid-out operands
+    int w_parts, db_parts;
+    long long dz_rows;               // rows of one part of the dz pass
+};
+
+template <class T>
+Plan plan_of(long long rows, int in, int out, bool pieces, bool slopes) {
+    Plan p = {};
+    const bool many = !few(rows, in > out ? in : out) || rows >= 4096;
+    int narrow_parts = 0, narrow_blocks = 0;
+    const bool is_narrow = visit_back<T>(out, in, [&](auto ob, auto ib) {
+        using M = Back<T, decltype(ob)::value, decltype(ib)::value>;
+        narrow_blocks = back_blocks<M>(rows, in, out);
+        narrow_parts = narrow_blocks * M::kSlices;
+    });
+    p.narrow = is_narrow && rows && (pieces || many);
+    p.stream = !p.narrow && rows && (in > 64 || out > 64) && in >= 16 && out >= 16 && !few(rows, in) && (pieces || many);
+    p.pad = (p.narrow || p.stream) && !pieces;
+    const Split sp = split_of(rows, in, out);
+    p.w_parts = p.narrow ? narrow_parts : sp.parts;
+    p.dz_rows = (rows + kDzParts - 1) / kDzParts;
+    const bool own_db = p.stream || p.pad;  // the bias gradient comes from the dz pass
+    p.db_parts = own_db ? (int)((rows + p.dz_rows - 1) / (p.dz_rows ? p.dz_rows : 1)) : p.narrow ? narrow_blocks : sp.parts;
+    auto take = [&](size_t bytes) { const size_t at = p.bytes; p.bytes += (bytes + 255) / 256 * 256; return at; };
+    p.dw = take((size_t)p.w_parts * in * out * 4);
+    p.db = take((size_t)p.db_parts * out * 4);
+    p.dz = take(own_db && (slopes || p.pad) ? (size_t)rows * whole_pieces<T>(out) * sizeof(T) : 0);
+    p.x = take(p.pad ? (size_t)rows * whole_pieces<T>(in) * sizeof(T) : 0);
+    p.w = take(p.pad ? (size_t)out * whole_pieces<T>(in) * sizeof(T) : 0);
+    return p;
+}
+
+template <class T>
+int pad(const void* from, long long ld, long long rows, int cols, T* to, hipStream_t s) {
+    const int pieces = (int)(whole_pieces<T>(cols) / Elem<T>::kE);
+    const long long blocks = (rows * pieces + 255) / 256;
+    linear_pad_kernel<T><<<(unsigned)(blocks < 4096 ? blocks : 4096), 256, 0, s>>>((const T*)from, ld, rows, cols, to, pieces);
+    return (int)hipGetLastError();
+}
+
+template <class T>
+int backward_any(LinearArgs a, hipStream_t s) {
+    constexpr int kE = Elem<T>::kE, kK = kPieces * kE;
+    const bool pieces = a.in % kE == 0 && a.out % kE == 0 && a.x_ld % kE == 0 && a.dy_ld % kE == 0 && a.w_ld % kE == 0 && aligned16(a.x) && aligned16(a.dy) && aligned16(a.slope) && aligned16(a.w);
+    const bool sums = a.dw || a.db;
+    if (!sums) {  // the input gradient alone needs no workspace
+        return a.rows ? product<T, kInput>(a, a.in, s) : 0;
+    }
+    const Plan p = plan_of<T>(a.rows, a.in, a.out, pieces, a.slope != nullptr);
+    char* const work = (char*)a.work;
+    float *const dw_work = (float*)(work + p.dw), *const db_work = (float*)(work + p.db);
+    int rc = 0;
+    if (p.stream || p.pad) {
+        T* const dz = a.slope || p.pad ? (T*)(work + p.dz) : nullptr;
+        if (dz || a.db) {
+            linear_dz_kernel<T><<<dim3((unsigned)p.db_parts, (a.out + 32 * kE - 1) / (32 * kE)), 256, 0, s>>>(a, dz, whole_pieces<T>(a.out), a.db ? db_work : nullptr, p.dz_rows);
+            if ((rc = (int)hipGetLastError())) return rc;
+        }
+        if (dz) { a.dy = dz; a.dy_ld = whole_pieces<T>(a.out); a.slope = nullptr; }
+        if (p.pad) {
+            if ((rc = pad<T>(a.x, a.x_ld, a.rows, a.in, (T*)(work + p.x), s))) return rc;
+            a.x = work + p.x; a.x_ld = whole_pieces<T>(a.in);
+        }
+        if (p.stream && p.pad && a.dx) {
+            if ((rc = pad<T>(a.w, a.w_ld, a.out, a.in, (T*)(work + p.w), s))) return rc;
+            a.w = work + p.w; a.w_ld = whole_pieces<T>(a.in);
+        }
+    }
+    a.work = dw_work;
+    if (p.narrow) {
+        LinearArgs b = a;
+        if (p.pad) b.db = nullptr;
+        visit_back<T>(a.out, a.in, [&](auto ob, auto ib) {
+            constexpr int OB = decltype(ob)::value, IB = decltype(ib)::value;
+            const int blocks = back_blocks<Back<T, OB, IB>>(a.rows, a.in, a.out);
+            linear_back_kernel<T, OB, IB><<<blocks, kBackThreads, 0, s>>>(b, db_work, blocks);
+            rc = (int)hipGetLastError();
+        });
+    } else if (p.stream) {
+        if (a.dx && (rc = stream_product<T, kInput>(a, a.in, s))) return rc;
+        if (a.dw) {
+            const long long part = ((a.rows + p.w_parts - 1) / p.w_parts + kK - 1) / kK * kK;
+            rc = stream<T, kWeight, 128, 128, 2, 2, 8, 2>(a, a.out, a.in, p.w_parts, part, s);
+        }
+    } else {
+        if (a.dx && a.rows && (rc = product<T, kInput>(a, a.in, s))) return rc;
+        rc = weight_grad<T>(a, db_work, split_of(a.rows, a.in, a.out), s);
+    }
+    if (rc) return rc;
+    const long long weights = (long long)a.out * a.in, all = (a.dw ? weights : 0) + (a.db ? a.out : 0);
+    linear_join_kernel<T><<<(unsigned)((all + 31) / 32), kJoinThreads, 0, s>>>(dw_work, db_work, (T*)a.dw, (T*)a.db, weights, a.out, p.w_parts, p.db_parts);
+    return (int)hipGetLastError();
+}
+
+template <class T>
+size_t work_bytes(long long rows, int in, int out) {  // (alignment and the activation are not known: room for any)
+    size_t most = 0;
+    for (int pieces = 0; pieces < 2; pieces++)
+        for (int slopes = 0; slopes < 2; slopes++) {
+            const size_t b = plan_of<T>(rows, in, out, pieces, slopes).bytes;
+            most = b > most ? b : most;
+        }
+    return most;
 }
 
 }  // namespace
 
-int linear_forward_launch(int dtype, const LinearArgs& a, hipStream_t s) {
-    if (!a.rows) return 0;
-    return dtype == DRONE_F32 ? forward_any<float>(a, s) : dtype == DRONE_BF16 ? forward_any<__bf16>(a, s) : forward_any<_Float16>(a, s);
-}
-int linear_backward_launch(int dtype, const LinearArgs& a, hipStream_t s) {
-    return dtype == DRONE_F32 ? backward_any<float>(a, s) : dtype == DRONE_BF16 ? backward_any<__bf16>(a, s) : backward_any<_Float16>(a, s);
-}
-size_t linear_work_bytes(int dtype, long long rows, int in, int out) {
-    // (whether the backward pass streams depends on alignment too: room for either)
-    const Split sp = split_of(rows, in, out);
-    const size_t dz = in > 64 && out > 64 && !few(rows, in) ? ((size_t)kDzParts * out + 4) * sizeof(float) + (size_t)rows * out * (dtype == DRONE_F32 ? 4 : 2) : 0;
-    return (size_t)sp.parts * ((size_t)in * out + out) * sizeof(float) + dz;
-}
+// One object file per element type (the Makefile compiles this file three times): DRONE_ELEM and its suffix.
+#define DRONE_NAME2(a, b) a##b
+#define DRONE_NAME(a, b) DRONE_NAME2(a, b)
+int DRONE_NAME(linear_forward_, DRONE_ELEM_NAME)(const LinearArgs& a, hipStream_t s) { return a.rows ? forward_any<DRONE_ELEM>(a, s) : 0; }
+int DRONE_NAME(linear_backward_, DRONE_ELEM_NAME)(const LinearArgs& a, hipStream_t s) { return backward_any<DRONE_ELEM>(a, s); }
+size_t DRONE_NAME(linear_work_, DRONE_ELEM_NAME)(long long rows, int in, int out) { return work_bytes<DRONE_ELEM>(rows, in, out); }
 
 }  // namespace drone

@@ -77,9 +77,16 @@ struct AdamwArgs {
 };
 
 // Launchers: 0, or the hipError_t of the launch. All check nothing: drone_policy.cpp has.
-int linear_forward_launch(int dtype, const LinearArgs& a, hipStream_t s);
-int linear_backward_launch(int dtype, const LinearArgs& a, hipStream_t s);
-size_t linear_work_bytes(int dtype, long long rows, int in, int out);
+#define DRONE_LINEAR_ENTRY(name)                                    \
+    int linear_forward_##name(const LinearArgs& a, hipStream_t s);  \
+    int linear_backward_##name(const LinearArgs& a, hipStream_t s); \
+    size_t linear_work_##name(long long rows, int in, int out);
+DRONE_LINEAR_ENTRY(f32)
+DRONE_LINEAR_ENTRY(bf16)
+DRONE_LINEAR_ENTRY(f16)
+inline int linear_forward_launch(int dtype, const LinearArgs& a, hipStream_t s) { return dtype == 0 ? linear_forward_f32(a, s) : dtype == 1 ? linear_forward_bf16(a, s) : linear_forward_f16(a, s); }
+inline int linear_backward_launch(int dtype, const LinearArgs& a, hipStream_t s) { return dtype == 0 ? linear_backward_f32(a, s) : dtype == 1 ? linear_backward_bf16(a, s) : linear_backward_f16(a, s); }
+inline size_t linear_work_bytes(int dtype, long long rows, int in, int out) { return dtype == 0 ? linear_work_f32(rows, in, out) : dtype == 1 ? linear_work_bf16(rows, in, out) : linear_work_f16(rows, in, out); }
 int norm_forward_launch(int dtype, const NormArgs& a, hipStream_t s);
 int norm_backward_launch(int dtype, const NormArgs& a, hipStream_t s);
 size_t norm_work_bytes(int dtype, long long rows, int width);
