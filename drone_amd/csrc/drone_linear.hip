@@ -1070,6 +1070,70 @@ __global__ __launch_bounds__(kBackThreads, 2) void linear_back_kernel(LinearArgs
     }
 }
 
+// ---- few rows: latency is everything. One 32 x 32 tile a workgroup, the reduction dealt out to its eight waves, fragments
+// straight from memory (all of a wave's loads under way at once, no LDS and no barrier before the sums are joined). ----
+template <class T, int ACT>
+__device__ __forceinline__ void few_forward(const LinearArgs& a, const float* sums, long long row0, int feat0) {
+    const int r = threadIdx.x >> 4, f = (threadIdx.x & 15) * 2;
+    const long long row = row0 + r;
+    if (row >= a.rows) return;
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        const int feat = feat0 + f + j;
+        if (feat >= a.out) continue;
+        float z = a.b ? to_f(((const T*)a.b)[feat]) : 0.f, s;
+#pragma unroll
+        for (int w = 0; w < 8; w++) z += sums[w * 1024 + r * 32 + f + j];
+        float v = activate<ACT, sizeof(T) == 4>(z, s);
+        if (a.slope) ((typename Elem<T>::Slope*)a.slope)[row * a.out + feat] = (typename Elem<T>::Slope)s;
+        if (a.res) v += to_f(((const T*)a.res)[row * a.res_ld + feat]);
+        ((T*)a.y)[row * a.y_ld + feat] = (T)v;
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(512) void linear_few_kernel(LinearArgs a, int tiles_n) {
+    constexpr int kE = Elem<T>::kE, kAhead = 4;
+    __shared__ float sums[8 * 1024];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, l32 = lane & 31;
+    const long long row0 = (long long)(blockIdx.x / tiles_n) * 32;
+    const int feat0 = (int)(blockIdx.x % tiles_n) * 32;
+    const long long row = row0 + l32 < a.rows ? row0 + l32 : a.rows - 1;
+    const int feat = feat0 + l32 < a.out ? feat0 + l32 : a.out - 1;
+    const T *x = (const T*)a.x + row * a.x_ld, *w = (const T*)a.w + feat * a.w_ld;
+    f32x16 acc = {};
+    const bool whole = a.in % kE == 0;
+    for (int k0 = wave * 2 * kE; k0 < a.in; k0 += 8 * 2 * kE * kAhead) {
+        u32x4 fx[kAhead], fw[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) {
+            const int k = k0 + i * 8 * 2 * kE + half * kE;
+            if (whole) {
+                const bool in = k < a.in;
+                const int at = in ? k : 0;
+                fx[i] = __builtin_bit_cast(u32x4, load_n<T, kE>(x + at, kE));
+                fw[i] = __builtin_bit_cast(u32x4, load_n<T, kE>(w + at, kE));
+                if (!in) fx[i] = fw[i] = u32x4{0, 0, 0, 0};
+            } else {
+                fx[i] = __builtin_bit_cast(u32x4, load_end<T, kE>(x, k, a.in));
+                fw[i] = __builtin_bit_cast(u32x4, load_end<T, kE>(w, k, a.in));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) mfma(acc, fw[i], fx[i], T{});
+    }
+#pragma unroll
+    for (int q = 0; q < 16; q++) sums[wave * 1024 + l32 * 32 + 8 * (q >> 2) + 4 * half + (q & 3)] = acc[q];
+    __syncthreads();
+    switch (a.act) {
+        case DRONE_ACTIVATION_RELU: few_forward<T, DRONE_ACTIVATION_RELU>(a, sums, row0, feat0); break;
+        case DRONE_ACTIVATION_TANH: few_forward<T, DRONE_ACTIVATION_TANH>(a, sums, row0, feat0); break;
+        case DRONE_ACTIVATION_SILU: few_forward<T, DRONE_ACTIVATION_SILU>(a, sums, row0, feat0); break;
+        case DRONE_ACTIVATION_GELU: few_forward<T, DRONE_ACTIVATION_GELU>(a, sums, row0, feat0); break;
+        default: few_forward<T, DRONE_ACTIVATION_NONE>(a, sums, row0, feat0);
+    }
+}
+
 // Joins the partial sums of the weight and bias gradients in a fixed order, 32 values a workgroup, eight threads a value:
 // every result is the same in every run.
 template <class T>
@@ -1149,6 +1213,11 @@ int stream(const LinearArgs& a, long long nrows, long long nfeat, int parts, lon
 template <class T, Product P>
 int stream_product(const LinearArgs& a, long long feats, hipStream_t s) {
     if (feats <= 64) return stream<T, P, 128, 64, 4, 1, 8, 2>(a, a.rows, feats, 1, 0, s);
+    // 256 x 256 tiles where they fill the card: half the loads from L2 for each product (65536 x 1024 x 1024 bf16: 179 us, 213
+    // with 128 x 128; deeper pipelines of 32-element steps: 190). f32 is bound by its matrix rate either way.
+    if constexpr (sizeof(T) == 2) {
+        if (feats >= 256 && (a.rows + 255) / 256 * ((feats + 255) / 256) >= 512 && (P == kForward ? a.in : a.out) >= 512) return stream<T, P, 256, 256, 4, 2, 8, 2>(a, a.rows, feats, 1, 0, s);
+    }
     return stream<T, P, 128, 128, 2, 2, 8, 2>(a, a.rows, feats, 1, 0, s);
 }
 
@@ -1207,12 +1276,19 @@ int forward_any(const LinearArgs& a, hipStream_t s) {
         const int rc = resident_any<T>(a, s);
         if (rc >= 0) return rc;
     }
+    const int tiles_n = (a.out + 31) / 32;
+    // One workgroup a CU at most: beyond, the tiled form's reuse wins (1 x 512 x 512 bf16: 4.8 against 7.0 us, 1024 x 20 x 64
+    // f32: 4.0 against 5.8; 2048 x 512 x 512 bf16, 1024 workgroups: 13.5 against 9.2).
+    if ((a.rows + 31) / 32 * tiles_n <= 256) {
+        linear_few_kernel<T><<<(unsigned)((a.rows + 31) / 32 * tiles_n), 512, 0, s>>>(a, tiles_n);
+        return (int)hipGetLastError();
+    }
     if (pieces && a.out > 32 && !few(a.rows, a.out)) return stream_product<T, kForward>(a, a.out, s);
     return product<T, kForward>(a, a.out, s);
 }
 
 // The class of a width in blocks of 32: 2, 4, 8 (f32: up to 4), 0 where the one-pass gradient does not reach. Wider pairs than
-// 16 blocks spill (131072 x 256 x 256 bf16 in one pass: 240 us; in three: 190).
+// 16 blocks spill (131072 x 256 x 256 bf16, forward and gradient: 301 us in one pass, 226 in three).
 template <class T>
 int blocks_of(int n) { return n <= 64 ? 2 : n <= 128 ? 4 : n <= 256 && sizeof(T) == 2 ? 8 : 0; }
 
