@@ -160,6 +160,17 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
     }
 };
 
+// Whether two row matrices of one allocation share an element (exact for equal leading dimensions, by address range else).
+bool overlap(const Tensor& a, const Tensor& b) {
+    if (!a.defined() || !b.defined() || !a.numel() || !b.numel() || !a.is_alias_of(b)) return false;
+    const int64_t d = (int64_t)((const char*)b.data_ptr() - (const char*)a.data_ptr()) / (int64_t)a.element_size(), la = ld(a), lb = ld(b);
+    const int64_t end_a = (a.size(0) - 1) * la + a.size(1), end_b = (b.size(0) - 1) * lb + b.size(1);
+    if (d >= end_a || -d >= end_b) return false;
+    if (la != lb) return true;
+    const int64_t c = ((d % la) + la) % la;  // b's first column as a counts them
+    return c < a.size(1) || c + b.size(1) > la;
+}
+
 Tensor linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, const std::string& activation, const OptTensor& residual, const OptTensor& out) {
     dtype_of(x, "x");
     const int act = activation_of(activation);
@@ -179,6 +190,9 @@ Tensor linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, cons
         TORCH_CHECK_VALUE(!learn, "out= cannot be differentiated: call under torch.no_grad()");
         const Tensor o = flat ? *out : out->view({x2.size(0), n});
         TORCH_CHECK_VALUE(good_rows(o), "out must have contiguous rows that do not overlap");
+        const bool in_place = r2.defined() && r2.data_ptr() == o.data_ptr() && ld(r2) == ld(o);
+        TORCH_CHECK_VALUE(!overlap(x2, o) && !overlap(w2, o) && !(b2.defined() && overlap(b2.unsqueeze(0), o)) && (in_place || !overlap(r2, o)),
+                          "out overlaps an input (only the residual may be updated in place)");
         linear_forward(x2, w2, b2, r2, act, o, Tensor());
         return *out;
     }

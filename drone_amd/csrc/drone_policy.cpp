@@ -13,6 +13,7 @@ struct OnDevice {
     DeviceRestore restore;
     bool ok;
     explicit OnDevice(int device) {
+        (void)hipGetLastError();  // an error an earlier call of someone else left is not this call's
         const hipError_t e = hipSetDevice(device);
         ok = e == hipSuccess;
         if (!ok) { set_err("hipSetDevice(%d) failed: %s", device, hipGetErrorString(e)); (void)hipGetLastError(); }
@@ -39,7 +40,7 @@ bool check_linear(const DroneLinear* c, const char* what) {
     if (c->struct_size != sizeof(DroneLinear)) return fail(what, "struct_size is not sizeof(DroneLinear)");
     if (!known(c->dtype)) return fail(what, "unknown dtype");
     if (c->activation < DRONE_ACTIVATION_NONE || c->activation > DRONE_ACTIVATION_GELU) return fail(what, "unknown activation");
-    if (c->rows < 0 || c->rows > 0x7fffffffLL) return fail(what, "rows must be 0 ... 2^31 - 1");
+    if (c->rows < 0 || c->rows > (1LL << 30)) return fail(what, "rows must be 0 ... 2^30");
     if (c->in_features < 1 || c->in_features > 65536 || c->out_features < 1 || c->out_features > 65536) return fail(what, "in_features and out_features must be 1 ... 65536");
     return true;
 }
@@ -61,7 +62,7 @@ bool check_norm(const DroneNorm* c, const char* what) {
     if (c->struct_size != sizeof(DroneNorm)) return fail(what, "struct_size is not sizeof(DroneNorm)");
     if (!known(c->dtype)) return fail(what, "unknown dtype");
     if (c->gate_kind < 0 || c->gate_kind > 2) return fail(what, "gate_kind must be 0, 1 or 2");
-    if (c->rows < 0 || c->rows > 0x7fffffffLL) return fail(what, "rows must be 0 ... 2^31 - 1");
+    if (c->rows < 0 || c->rows > (1LL << 30)) return fail(what, "rows must be 0 ... 2^30");
     if (c->width < 1 || c->width > 4096) return fail(what, "width must be 1 ... 4096");
     if (!(c->eps >= 0.f)) return fail(what, "eps must not be negative");
     if (c->gate_kind && !c->gate) { if (c->rows || c->gate_kind == 1) return fail(what, "gate is NULL"); }
@@ -94,11 +95,11 @@ bool check_adamw(const DroneAdamW* c, const char* what) {
     if (!known(c->dtype)) return fail(what, "unknown dtype");
     if (c->count < 0 || (c->count && !c->tensors)) return fail(what, "tensors is NULL");
     for (int i = 0; i < c->count; i++)
-        if (c->tensors[i].elements < 0 || c->tensors[i].elements > (1LL << 40)) return fail(what, "a tensor's elements must be 0 ... 2^40");
+        if (c->tensors[i].elements < 0 || c->tensors[i].elements > (1LL << 34)) return fail(what, "a tensor's elements must be 0 ... 2^34");
     return true;
 }
 
-// One launch's share of the tensors: up to kAdamwTensors of them, at most 2^30 chunks. Returns how many it took.
+// One launch's share of the tensors: up to kAdamwTensors of them, at most 2^23 chunks (one tensor may be as many). Returns how many it took.
 int fill_adamw(const DroneAdamW* c, int from, AdamwArgs* a) {
     const uintptr_t align = 15;
     long long chunks = 0;
@@ -108,7 +109,7 @@ int fill_adamw(const DroneAdamW* c, int from, AdamwArgs* a) {
         const DroneAdamWTensor& s = c->tensors[i];
         if (!s.elements) continue;
         const long long more = chunks_of(s.elements);
-        if (a->count && chunks + more > (1LL << 30)) break;
+        if (a->count && chunks + more > (1LL << 23)) break;
         AdamwTensor& t = a->t[a->count++];
         t.p = s.param; t.g = s.grad; t.m = s.exp_avg; t.v = s.exp_avg_sq; t.master = s.master;
         t.n = s.elements;
@@ -215,7 +216,6 @@ int drone_adamw_step(const DroneAdamW* c, void* stream) {
     for (int i = 0; i < c->count; i++) {
         const DroneAdamWTensor& t = c->tensors[i];
         if (!t.elements) continue;
-        if (t.elements > (1LL << 40)) return fail(what, "a tensor is too large"), -1;
         if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq) return fail(what, "a tensor's pointer is NULL"), -1;
         if ((c->dtype != DRONE_F32) != (t.master != nullptr)) return fail(what, "16-bit tensors need a 32-bit master, DRONE_F32 ones have none"), -1;
         if (odd(t.param, m) || odd(t.grad, m) || odd(t.exp_avg, 3) || odd(t.exp_avg_sq, 3) || odd(t.master, 3)) return fail(what, "a pointer is not aligned to its elements"), -1;

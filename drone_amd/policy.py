@@ -90,18 +90,25 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("lr, eps and weight_decay must not be negative, betas must be in [0, 1)")
         if max_grad_norm is not None and not max_grad_norm > 0:
             raise ValueError("max_grad_norm must be positive (None: no clipping)")
-        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, max_grad_norm=max_grad_norm))
         self.grad_norm = []
-        for group in self.param_groups:
-            if len({p.dtype for p in group["params"]}) != 1 or len({p.device for p in group["params"]}) != 1:
-                raise ValueError("the parameters of a group must have one type and one device")
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, max_grad_norm=max_grad_norm))
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        try:
             for p in group["params"]:
                 _check_parameter(p)
-            group["step"] = torch.zeros(1, dtype=torch.int32, device=group["params"][0].device)
-            for p in group["params"]:
-                self.state[p] = {"exp_avg": torch.zeros(p.shape, dtype=torch.float32, device=p.device), "exp_avg_sq": torch.zeros(p.shape, dtype=torch.float32, device=p.device)}
-                if p.dtype != torch.float32:
-                    self.state[p]["master"] = p.detach().float()
+            if len({p.dtype for p in group["params"]}) != 1 or len({p.device for p in group["params"]}) != 1:
+                raise ValueError("the parameters of a group must have one type and one device")
+        except Exception:
+            self.param_groups.pop()
+            raise
+        group["step"] = torch.zeros(1, dtype=torch.int32, device=group["params"][0].device)
+        for p in group["params"]:
+            self.state[p] = {"exp_avg": torch.zeros(p.shape, dtype=torch.float32, device=p.device), "exp_avg_sq": torch.zeros(p.shape, dtype=torch.float32, device=p.device)}
+            if p.dtype != torch.float32:
+                self.state[p]["master"] = p.detach().float()
 
     @torch.no_grad()
     def load_state_dict(self, state_dict):

@@ -382,8 +382,9 @@ int drone_vec_copy_to_host(DroneVec* v, void* host_dst, const void* device_src, 
  * (NULL only for DRONE_ACTIVATION_NONE) with dy [rows][out] and writes those of
  *   dx = dz W,   dweight = dz^T x,   dbias = sum of dz over the rows,   dz = dy * slope
  * that are not NULL (dweight [out][in] and dbias [out] dense); the residual's gradient is dy itself. y may be the residual
- * (same pointer and leading dimension); no other output may overlap an input. rows 0 ... 2^31 - 1 (0: sums are zero),
- * in / out 1 ... 65536. Backward with dweight or dbias needs drone_linear_workspace bytes at `workspace` (16-byte aligned). */
+ * (same pointer and leading dimension); no other output may overlap an input. rows 0 ... 2^30 (0: sums are zero),
+ * in / out 1 ... 65536. Backward with dweight or dbias needs drone_linear_workspace bytes at `workspace` (16-byte aligned):
+ * partial sums, and for wide or odd layers dz and copies laid out in whole pieces (up to about rows (in + out) elements). */
 typedef struct DroneLinear {
     uint32_t struct_size; /* = sizeof(DroneLinear) */
     int32_t device, dtype, activation;
@@ -428,7 +429,7 @@ uint64_t drone_norm_workspace(const DroneNorm* call);
  * DRONE_F32), each dense with `elements` values. `step` (device, one int32) counts the steps done: the call adds 1 and t is
  * the result, so a captured call replays with an advancing t (lr and the rest stay those of the capture). `grad_norm`
  * (device, one f32) or NULL receives the norm before clipping. `tensors` is host memory, read during the call. No tensor
- * may appear twice. drone_adamw_workspace bytes at `workspace`. */
+ * may appear twice; elements 0 ... 2^34. drone_adamw_workspace bytes at `workspace`. */
 typedef struct DroneAdamWTensor {
     void* param;
     const void* grad;

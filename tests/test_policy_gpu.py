@@ -214,14 +214,38 @@ def test_linear_is_the_same_every_time(t):
     assert torch.equal(first[0], again[0]) and all(torch.equal(first[1][g], again[1][g]) for g in first[1])
 
 
-def test_linear_only_the_gradients_asked_for():
+@pytest.mark.parametrize("m, k, n", [(300, 33, 65), (5000, 64, 64), (9001, 30, 100), (20001, 264, 136), (20001, 333, 129)])
+@pytest.mark.parametrize("act", ["relu", "none"])
+def test_linear_only_the_gradients_asked_for(m, k, n, act):
+    """Every subset of the three, in each of the gradient's forms (tiled, one pass, streamed; laid out or as it is). The
+    input gradient alone takes the tiled form: the same sums in another order, held to the tolerance."""
     for t in TYPES:
+        x, w, b, _, dy = linear_case(m, k, n, t, act, res=False)
+        full = torch.autograd.grad(policy.linear(x, w, b, act), [x, w, b], dy)
         for needs in range(1, 8):
-            x, w, b, _, dy = linear_case(300, 33, 65, t, "relu", res=False)
-            full = torch.autograd.grad(policy.linear(x, w, b, "relu"), [x, w, b], dy)
             vs = [v.detach().requires_grad_(bool(needs >> i & 1)) for i, v in enumerate((x, w, b))]
-            got = torch.autograd.grad(policy.linear(*vs, "relu"), [v for v in vs if v.requires_grad], dy)
-            assert all(torch.equal(a, c) for a, c in zip(got, [f for f, v in zip(full, vs) if v.requires_grad])), (t, needs)
+            got = torch.autograd.grad(policy.linear(*vs, act), [v for v in vs if v.requires_grad], dy)
+            want = [f for f, v in zip(full, vs) if v.requires_grad]
+            if needs == 1:
+                ref = linear_reference(x.detach(), w.detach(), b.detach(), None, dy, act)["dx"]
+                close(got[0], *ref, "dx alone")
+            else:
+                assert all(torch.equal(a, c) for a, c in zip(got, want)), (t, needs)
+
+
+def test_linear_refuses_overlapping_out():
+    x, w = rand(40, 32, seed=1), rand(32, 32, seed=2)
+    block = torch.zeros(40, 80, device="cuda")
+    with torch.no_grad():
+        for kw in (dict(out=x), dict(residual=block[:, :32], out=block[:, 8:40])):
+            with pytest.raises(ValueError, match="overlaps"):
+                policy.linear(x, w, **kw)
+        inside = block[:, :32].copy_(x)
+        with pytest.raises(ValueError, match="overlaps"):
+            policy.linear(inside, w, out=block[:, 31:63])
+        assert torch.equal(policy.linear(inside, w, out=block[:, 32:64]), policy.linear(x, w))
+        with pytest.raises(ValueError, match="overlaps"):
+            policy.linear(x[:32], w, out=w)
 
 
 @pytest.mark.parametrize("act", ["none", "tanh", "silu", "gelu"])
@@ -741,3 +765,9 @@ def test_optimizer_groups_state_and_skipped_parameters():
     assert all(torch.equal(p, q) for p, q in zip(ps, after))
     with pytest.raises(ValueError, match="one type"):
         policy.AdamW([ps[0], ps[2]])
+    late = torch.nn.Parameter(rand(5, seed=8))
+    opt.add_param_group({"params": [late]})  # a group added later has its state too
+    late.grad = torch.ones_like(late)
+    was = late.detach().clone()
+    opt.step()
+    assert not torch.equal(late, was) and opt.param_groups[2]["step"].item() == 1
