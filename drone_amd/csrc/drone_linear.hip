@@ -1,8 +1,17 @@
 // drone_linear.hip — y = act(x W^T + b) + residual and its gradient, for the policy networks a device-resident learner runs
-// between env steps. Three products, one tiled kernel:
+// between env steps. Three products:
 //   forward  Y[m][n]  = sum_k X[m][k] W[n][k]      bias, activation, residual and act'(z) in the epilogue
-//   input    DX[m][k] = sum_n DZ[m][n] W[n][k]     DZ = dy * act'(z), formed while the tile is staged
+//   input    DX[m][k] = sum_n DZ[m][n] W[n][k]     DZ = dy * act'(z)
 //   weight   DW[n][k] = sum_m DZ[m][n] X[m][k]     split over m, partial sums joined in a fixed order; db rides along
+// A policy's layers have many rows and few columns, so most of them are bound by memory, small ones by latency, and only wide
+// ones by the matrix cores. The forms, chosen by size, type and alignment alone (measured on one MI355X; a large copy moves
+// 5.1 TB/s there, a large product runs at 1 310 TFLOP/s bf16 and 153 f32):
+//   linear_kernel           any size and alignment: tiles through registers into LDS, dz formed on the way
+//   linear_few_kernel       few rows: one 32 x 32 tile a workgroup, the reduction dealt out to its waves
+//   linear_resident_kernel  reductions of at most 1 KiB a row: weights in registers, rows streaming through LDS
+//   linear_stream_kernel    whole 16-byte pieces: tiles straight from memory to LDS (wide layers, wide gradients)
+//   linear_back_kernel      narrow layers: the whole gradient in one pass over the rows
+// Odd widths take the streaming gradients too, on operands laid out in whole pieces (linear_dz_kernel, linear_pad_kernel).
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -784,7 +793,7 @@ __global__ __launch_bounds__(kResidentWaves * 64, 2 * PER_CU) void linear_reside
 // dz = dy * slope, rounded once to T, into rows of whole pieces (or nowhere: dz is dy), and the bias gradient's partial
 // sums of the 32-bit values: thread (c, g) of a workgroup owns piece c of a strip of kStrip pieces and every kGroups-th of the
 // workgroup's rows.
-template <class T>
+template <class T, bool WHOLE>
 __global__ __launch_bounds__(256) void linear_dz_kernel(LinearArgs a, T* dz, long long dz_ld, float* partial, long long rows_part) {
     using Slope = typename Elem<T>::Slope;
     constexpr int kE = Elem<T>::kE, kStrip = 32, kGroups = 8;
@@ -796,13 +805,12 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(LinearArgs a, T* dz, lon
     if (left > 0)
 #pragma unroll 4
         for (long long r = row0 + g; r < row1; r += kGroups) {
-            const bool whole = a.out % kE == 0;  // the same for the launch
-            const auto v = whole ? load_n<T, kE>((const T*)a.dy + r * a.dy_ld + col, kE) : load_end<T, kE>((const T*)a.dy + r * a.dy_ld, col, a.out);
+            const auto v = WHOLE ? load_n<T, kE>((const T*)a.dy + r * a.dy_ld + col, kE) : load_end<T, kE>((const T*)a.dy + r * a.dy_ld, col, a.out);
             float f[kE];
 #pragma unroll
             for (int e = 0; e < kE; e++) f[e] = to_f(v.e[e]);
             if (a.slope) {
-                const auto q = whole ? load_n<Slope, kE>((const Slope*)a.slope + r * a.out + col, kE) : load_end<Slope, kE>((const Slope*)a.slope + r * a.out, col, a.out);
+                const auto q = WHOLE ? load_n<Slope, kE>((const Slope*)a.slope + r * a.out + col, kE) : load_end<Slope, kE>((const Slope*)a.slope + r * a.out, col, a.out);
 #pragma unroll
                 for (int e = 0; e < kE; e++) f[e] *= to_f(q.e[e]);
             }
@@ -1376,7 +1384,9 @@ int backward_any(LinearArgs a, hipStream_t s) {
     if (p.stream || p.pad) {
         T* const dz = a.slope || p.pad ? (T*)(work + p.dz) : nullptr;
         if (dz || a.db) {
-            linear_dz_kernel<T><<<dim3((unsigned)p.db_parts, (a.out + 32 * kE - 1) / (32 * kE)), 256, 0, s>>>(a, dz, whole_pieces<T>(a.out), a.db ? db_work : nullptr, p.dz_rows);
+            const dim3 grid((unsigned)p.db_parts, (a.out + 32 * kE - 1) / (32 * kE));
+            if (a.out % kE == 0) linear_dz_kernel<T, true><<<grid, 256, 0, s>>>(a, dz, whole_pieces<T>(a.out), a.db ? db_work : nullptr, p.dz_rows);
+            else linear_dz_kernel<T, false><<<grid, 256, 0, s>>>(a, dz, whole_pieces<T>(a.out), a.db ? db_work : nullptr, p.dz_rows);
             if ((rc = (int)hipGetLastError())) return rc;
         }
         if (dz) { a.dy = dz; a.dy_ld = whole_pieces<T>(a.out); a.slope = nullptr; }

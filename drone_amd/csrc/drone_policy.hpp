@@ -73,7 +73,7 @@ struct AdamwArgs {
     float* norm;        // [1] or null
     int* step;
     float lr, decay, b1, b2, rest1, rest2, eps, max_norm;  // decay = 1 - lr wd, rest = 1 - b: formed in 64 bits (1 - 0.999f is 1e-5 off)
-    double b1d, b2d;
+    float log_b1, log_b2;
 };
 
 // Launchers: 0, or the hipError_t of the launch. All check nothing: drone_policy.cpp has.
@@ -92,6 +92,8 @@ int norm_backward_launch(int dtype, const NormArgs& a, hipStream_t s);
 size_t norm_work_bytes(int dtype, long long rows, int width);
 int adamw_norm_launch(int dtype, const AdamwArgs& a, int blocks, hipStream_t s);
 int adamw_update_launch(int dtype, const AdamwArgs& a, hipStream_t s);
+int adamw_small_launch(int dtype, const AdamwArgs& a, hipStream_t s);
+constexpr int kAdamwSmall = 8;      // chunks up to which one workgroup does the whole step in one launch
 constexpr int kAdamwChunk = 2048;   // elements one workgroup updates
 constexpr int kAdamwParts = 512;    // partial sums of one norm launch at most
 

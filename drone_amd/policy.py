@@ -61,7 +61,8 @@ def norm_residual(x, block=None, *, gate=None, scale=1.0, post_weight=None, pre_
 
 @torch.no_grad()
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, max_grad_norm=None, masters=None):
-    """One AdamW step over all tensors, in place, two launches; returns the gradients' global norm before clipping
+    """One AdamW step over all tensors, in place, two launches (one where all tensors
+    together are a few thousand values); returns the gradients' global norm before clipping
     (``[1]`` float32 on the device). ``max_grad_norm``: scale the gradients by ``min(1, max_grad_norm / (norm + 1e-6))``.
 
     params and grads of one type; exp_avgs, exp_avg_sqs float32; 16-bit params need float32 ``masters`` (the params are
