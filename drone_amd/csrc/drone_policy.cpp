@@ -2,6 +2,7 @@
 // argument checks, device and stream, then the launchers of drone_linear.hip / drone_norm.hip / drone_adamw.hip.
 #include "drone_policy.hpp"
 
+#include <cfloat>
 #include <cmath>
 
 #include "drone_vec_impl.hpp"
@@ -212,7 +213,9 @@ int drone_adamw_step(const DroneAdamW* c, void* stream) {
     if (!check_adamw(c, what)) return -1;
     if (!c->step || odd(c->step, 3)) return fail(what, "step is NULL or misaligned"), -1;
     if (!(c->beta1 >= 0 && c->beta1 < 1 && c->beta2 >= 0 && c->beta2 < 1)) return fail(what, "beta1 and beta2 must be in [0, 1)"), -1;
-    if (!(c->lr >= 0) || !(c->eps >= 0) || !(c->weight_decay >= 0)) return fail(what, "lr, eps and weight_decay must not be negative"), -1;
+    if (!(c->lr >= 0) || !(c->weight_decay >= 0)) return fail(what, "lr and weight_decay must not be negative"), -1;
+    // the update multiplies m by rcp(sqrt(v) + eps) of the hardware, which take denormals for 0: without eps that is infinite
+    if (!((float)c->eps >= FLT_MIN)) return fail(what, "eps must be positive (a normal 32-bit number)"), -1;
     if (c->max_grad_norm != c->max_grad_norm) return fail(what, "max_grad_norm is not a number"), -1;
     const uintptr_t m = elem_mask(c->dtype);
     for (int i = 0; i < c->count; i++) {

@@ -87,8 +87,8 @@ class AdamW(torch.optim.Optimizer):
     group's. ``lr`` and the rest are read at every call (a captured step keeps those of its capture)."""
 
     def __init__(self, params, lr=3e-4, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, max_grad_norm=None):
-        if lr < 0 or eps < 0 or weight_decay < 0 or not all(0 <= b < 1 for b in betas):
-            raise ValueError("lr, eps and weight_decay must not be negative, betas must be in [0, 1)")
+        if lr < 0 or weight_decay < 0 or not eps > 0 or not all(0 <= b < 1 for b in betas):
+            raise ValueError("lr and weight_decay must not be negative, eps must be positive, betas in [0, 1)")
         if max_grad_norm is not None and not max_grad_norm > 0:
             raise ValueError("max_grad_norm must be positive (None: no clipping)")
         self.grad_norm = []

@@ -89,7 +89,7 @@ def test_norm_backward_refuses(hip, over, why):
 @pytest.mark.parametrize("over, tensor, why", [
     (dict(struct_size=8), {}, "struct_size"), (dict(dtype=9), {}, "unknown dtype"), (dict(count=-1), {}, "tensors"), (dict(tensors=None), {}, "tensors"),
     (dict(step=None), {}, "step"), (dict(step=P + 1), {}, "step"), (dict(beta1=1.0), {}, "beta"), (dict(beta2=-0.1), {}, "beta"), (dict(beta2=float("nan")), {}, "beta"),
-    (dict(lr=-1.0), {}, "lr"), (dict(eps=float("nan")), {}, "eps"), (dict(weight_decay=-1.0), {}, "weight_decay"), (dict(max_grad_norm=float("nan")), {}, "max_grad_norm"),
+    (dict(lr=-1.0), {}, "lr"), (dict(eps=float("nan")), {}, "eps"), (dict(eps=0.0), {}, "eps"), (dict(eps=1e-46), {}, "eps"), (dict(weight_decay=-1.0), {}, "weight_decay"), (dict(max_grad_norm=float("nan")), {}, "max_grad_norm"),
     ({}, dict(elements=-1), "elements"), ({}, dict(elements=1 << 41), "elements"), ({}, dict(grad=None), "NULL"), ({}, dict(master=P), "master"), (dict(dtype=1), {}, "master"),
     ({}, dict(exp_avg=P + 2), "not aligned"), (dict(workspace=None), {}, "drone_adamw_workspace"), (dict(workspace_bytes=8), {}, "drone_adamw_workspace")])
 def test_adamw_refuses(hip, over, tensor, why):
@@ -143,3 +143,6 @@ def test_cpu_tensors_are_refused(native):
         policy.AdamW([torch.nn.Parameter(w)], lr=-1.0)
     with pytest.raises(ValueError, match="must be positive"):
         policy.AdamW([torch.nn.Parameter(w)], max_grad_norm=0.0)
+    for eps in (0.0, -1e-8, float("nan")):
+        with pytest.raises(ValueError, match="eps"):
+            policy.AdamW([torch.nn.Parameter(w)], eps=eps)

@@ -514,6 +514,15 @@ def test_adamw_sizes(t, shapes):
     check_adamw(s, None, "second", lr=0.0)
 
 
+def test_adamw_extreme_settings():
+    """Moments that forget at once, no decay, a large eps, a count far along: the bias corrections' two ends."""
+    for t, over in ((torch.float32, dict(betas=(0.0, 0.5), eps=1e-3)), (torch.bfloat16, dict(betas=(0.0, 0.0), weight_decay=0.0)), (torch.float32, dict(betas=(0.99, 0.9999)))):
+        s = adamw_case([(70, 33), (5,)], t)
+        check_adamw(s, 0.5, str(over), **over)
+        s["step"].fill_(2_000_000)
+        check_adamw(s, None, f"late {over}", **over)
+
+
 def test_adamw_large_total():
     """Enough values that the norm's partial sums are spread over all its workgroups, many chunks each."""
     check_adamw(adamw_case([(1024, 1024), (1024,), (3000, 999)], torch.bfloat16), 1.0, "large")
