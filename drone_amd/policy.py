@@ -41,7 +41,8 @@ def linear(x, weight, bias=None, activation="none", residual=None, out=None):
     """``act(x @ weight.T + bias) + residual`` in one launch, differentiable (once) in all four.
 
     x ``[..., in]``, weight ``[out, in]``, bias ``[out]``, residual ``[..., out]``, one type (float32, bfloat16, float16)
-    and one GPU; activation: none, relu, tanh, silu, gelu (the erf form). Sums are 32-bit, the result is rounded once.
+    and one GPU; activation: none, relu, tanh, silu, gelu (the erf form). Sums are 32-bit, the result is rounded once; calls of
+    one shape give the same bits, another number of rows may sum in another order.
     ``out``: a tensor to write instead of a new one (the env's action buffer), ``[..., out]`` with contiguous rows; only
     where nothing is differentiated; it may be the residual. Rows may be a strided view; anything else is copied first."""
     return _native().linear(x, weight, bias, activation, residual, out)
