@@ -281,12 +281,12 @@ void leave_zero_copy(DroneVec* v) {
 // Which caller host buffers may be pinned. hipHostRegister works at page granularity, and on ROCm 7 registering (and
 // later unregistering) a range that shares a page with OTHER heap memory breaks the runtime's own on-the-fly pinning of
 // pageable copy destinations on that page: a later hipMemcpy / torch .cpu() into a neighbouring allocation dies with
-// "Memory access fault by GPU ... on address <heap address>" (tools/debug/pageable_copy_stress.py reproduces it with
-// plain HIP calls; ~1 in 12 runs of this repo's GPU test suite hit it before this rule). Round 5 found the rule of rounds
+// "Memory access fault by GPU ... on address <heap address>" (seen with plain HIP calls
+// too; ~1 in 12 runs of this repo's GPU test suite hit it before this rule). Round 5 found the rule of rounds
 // 3-4 — "starts on a page boundary and spans whole pages" — still too generous: such a block INSIDE the malloc heap (a
 // numpy array that happens to start on a page boundary, a posix_memalign block) owns its pages but not its mapping, and
 // when the heap around it is trimmed or reused while the GPU writes the registered pages the same fault appears ("Write
-// access to a read-only page": tools/debug/heap_interior_registration_stress.py, library-free; two of eight soak runs died
+// access to a read-only page", seen without this library too; two of eight soak runs died
 // of it once heap-buffer handles took the zero-copy transports more often). A mapping of its own (mmap, POSIX shm) under
 // the same stress never faults. The library cannot tell the two apart, so alignment alone no longer suffices: a buffer is
 // registered only when the CALLER vouches for it (cfg.host_pages_exclusive: every buffer is a mapping of its own, page-

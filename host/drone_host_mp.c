@@ -49,7 +49,7 @@
  * vouches for, so that the library may pin it for the zero-copy transport. */
 static void* page_alloc(size_t bytes) {
     /* a mapping of its own (round 5: a posix_memalign block owns its pages but lies inside the malloc heap, and registered heap
-     * pages fault when the heap around them is trimmed while the GPU writes them: tools/debug/heap_interior_registration_stress.py) */
+     * pages fault when the heap around them is trimmed while the GPU writes them) */
     const size_t span = bytes ? (bytes + 4095) / 4096 * 4096 : 4096;
     void* p = mmap(NULL, span, PROT_READ | PROT_WRITE, MAP_PRIVATE | MAP_ANONYMOUS, -1, 0);
     if (p == MAP_FAILED) return NULL;

@@ -70,10 +70,10 @@ typedef struct DroneConfig {
      * else gets pinned stand-ins or is copied through pageable transfers and is never registered. Why the caller has to say
      * so: on ROCm 7, hipHostRegister / hipHostUnregister of a range that SHARES a page with other heap memory breaks the
      * runtime's own on-the-fly pinning of pageable copy destinations on that page ("Memory access fault by GPU ... on address
-     * <heap address>", tools/debug/pageable_copy_stress.py reproduces it without this library) — and (round 5) a block that
+     * <heap address>", seen without this library too) — and (round 5) a block that
      * owns its pages but lies INSIDE the malloc heap (posix_memalign, an array that happens to be page-aligned) faults the
      * same way once the heap around it is trimmed or reused while the GPU writes it
-     * (tools/debug/heap_interior_registration_stress.py); a mapping of its own never does. Rounds 3-4 registered any
+     * (seen without this library too); a mapping of its own never does. Rounds 3-4 registered any
      * page-aligned whole-page buffer unasked; the library cannot tell the two kinds apart, so it no longer does. */
     int32_t host_pages_exclusive;
     /* How the device keeps the state (round 4: the choice is part of the handle's declared contract, not only of
