@@ -215,6 +215,8 @@ __global__ __launch_bounds__(kThreads) void norm_backward_kernel(NormArgs a) {
     for (long long row0 = first; row0 < a.rows; row0 += step) {
         const long long row = row0 + threadIdx.x / TPR;
         const int width = row < a.rows ? a.width : 0;
+        // 1 / rms of the row; 0 behind the last one, whose zeros may add nothing to the column sums (without eps: 0 * inf)
+        auto inverse = [&](float squares) { return width ? 1.f / sqrtf(squares * inv_width + a.eps) : 0.f; };
         float r[NP][kE], nb[NP][kE], s[NP][kE], dh[NP][kE], d_[NP][kE], f[kE], sum = 0.f;
 #pragma unroll
         for (int i = 0; i < NP; i++) {
@@ -233,7 +235,7 @@ __global__ __launch_bounds__(kThreads) void norm_backward_kernel(NormArgs a) {
         if (row0 + step < a.rows) ask(row + step);
         float inv_b = 0.f;
         if (a.block) {
-            inv_b = 1.f / sqrtf(row_sum<TPR>(sum, join) * inv_width + a.eps);
+            inv_b = inverse(row_sum<TPR>(sum, join));
 #pragma unroll
             for (int i = 0; i < NP; i++) {
                 if (a.post) unpack<T>(w_post[i], f);
@@ -254,7 +256,7 @@ __global__ __launch_bounds__(kThreads) void norm_backward_kernel(NormArgs a) {
                 gr += r[i][e] * dh[i][e] * (a.pre ? f[e] : 1.f);
             }
         }
-        const float inv_r = 1.f / sqrtf(row_sum<TPR>(rr, join) * inv_width + a.eps);
+        const float inv_r = inverse(row_sum<TPR>(rr, join));
         const float mean_gr = row_sum<TPR>(gr, join) * inv_width * inv_r;  // mean(dh * pre * n(r))
         float ub = 0.f;
 #pragma unroll
