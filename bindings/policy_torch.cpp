@@ -88,6 +88,10 @@ int activation_of(const std::string& name) {
 
 Tensor workspace(uint64_t bytes, const Tensor& x) { return at::empty({(int64_t)bytes}, x.options().dtype(at::kByte)); }
 
+// What a call has written in place, by address: autograd's version counter has to move, so that a backward pass through a
+// graph that saved the tensor fails as it does behind torch's own in-place operators.
+void written(const Tensor& t) { if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version(); }
+
 // The gradients as a second differentiation has to see them: there is none.
 variable_list once(variable_list grads, const char* what) {
     if (!at::GradMode::is_enabled()) return grads;
@@ -187,13 +191,14 @@ Tensor linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, cons
     const Tensor x2 = rows_of(x), w2 = rows_of(weight), b2 = has(bias) ? bias->contiguous() : Tensor(), r2 = has(residual) ? rows_of(*residual) : Tensor();
     if (has(out)) {
         check("out", *out, shape, x);
-        TORCH_CHECK_VALUE(!learn, "out= cannot be differentiated: call under torch.no_grad()");
+        TORCH_CHECK_VALUE(!learn && !(at::GradMode::is_enabled() && out->requires_grad()), "out= cannot be differentiated: call under torch.no_grad()");
         const Tensor o = flat ? *out : out->view({x2.size(0), n});
         TORCH_CHECK_VALUE(good_rows(o), "out must have contiguous rows that do not overlap");
         const bool in_place = r2.defined() && r2.data_ptr() == o.data_ptr() && ld(r2) == ld(o);
         TORCH_CHECK_VALUE(!overlap(x2, o) && !overlap(w2, o) && !(b2.defined() && overlap(b2.unsqueeze(0), o)) && (in_place || !overlap(r2, o)),
                           "out overlaps an input (only the residual may be updated in place)");
         linear_forward(x2, w2, b2, r2, act, o, Tensor());
+        written(*out);
         return *out;
     }
     Tensor y;
@@ -357,6 +362,9 @@ Tensor adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& 
     c.workspace = ptr(work);
     c.workspace_bytes = work.numel();
     run(lib.adamw_step(&c, stream_of(first)));
+    for (const auto* list : {&params, &exp_avgs, &exp_avg_sqs}) for (const Tensor& t : *list) written(t);
+    if (masters) for (const Tensor& t : *masters) written(t);
+    written(step);
     return norm;
 }
 

@@ -154,6 +154,8 @@ class Drone:
                 own[0].copy_(bufs.actions[K - 1])
                 for mine, block in zip(own[1][1:], (bufs.rewards, bufs.terminals, bufs.truncations)):
                     mine.copy_(block[K - 1])
+            # the kernels wrote by address: a graph that saved one of these tensors must not be differentiated after this
+            torch.autograd.graph.increment_version((bufs.observations, bufs.actions, bufs.rewards, bufs.terminals, bufs.truncations, *own[1]))
         finally:
             vec.bind_actions(own[0])
             vec.bind_outputs(*own[1])

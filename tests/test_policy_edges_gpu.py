@@ -1,8 +1,10 @@
 """The policy operators at the edges of what they allow: calls that the other tests do not make, each against 64-bit
 formulas, against the same work done another way, or refused."""
 import pytest
+import torch
 
-from test_policy_gpu import TYPES, check_norm, norm_case
+from drone_amd import policy
+from test_policy_gpu import TYPES, check_norm, linear_case, norm_case, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -16,3 +18,68 @@ def test_norm_without_eps(t, gate, eps, m, c):
     """eps = 0 (and one that 32 bits round to 0) for rows that are not zero: threads behind the last row, of which every
     width class has some at these row counts, add nothing to the sums over the rows."""
     check_norm(*norm_case(m, c, t, gate), 0.5, eps, f"{m}x{c} {gate} eps={eps}")
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_a_graph_from_before_the_step_is_refused(t):
+    """adamw_step writes in place: a backward pass through a graph that saved the old weights has to fail, as it does with
+    torch's own optimizers, and not to take the new ones."""
+    x, w, b, _, dy = linear_case(50, 24, 32, t, "tanh", res=False)
+    y = policy.linear(x, w, b, "tanh")
+    r, h = policy.norm_residual(y, pre_weight=b)
+    opt = policy.AdamW([w, b], lr=1e-2)
+    w.grad, b.grad = torch.ones_like(w), torch.ones_like(b)
+    written = [w, b, opt.param_groups[0]["step"]] + [v for p in (w, b) for v in opt.state[p].values()]
+    before = [v._version for v in written]
+    read = (w.grad._version, b.grad._version)
+    opt.step()
+    assert all(v._version > n for v, n in zip(written, before)) and (w.grad._version, b.grad._version) == read
+    for out in (y, h):
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.backward(torch.ones_like(out), retain_graph=True)
+    again = policy.linear(x, w, b, "tanh")  # a graph built after it goes through
+    torch.autograd.grad(again, [x, w, b], dy)
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_out_into_a_saved_tensor_is_refused(t):
+    x, w, b, _, dy = linear_case(50, 24, 32, t, "none", res=False)
+    saved = x.detach().clone()
+    y = policy.linear(saved, w, b)
+    with torch.no_grad():
+        policy.linear(saved.new_ones(50, 8), saved.new_ones(24, 8), out=saved)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(dy)
+    with torch.inference_mode():  # tensors that keep no version are written all the same
+        free = torch.zeros(50, 32, dtype=t, device="cuda")
+        assert torch.equal(policy.linear(x, w, b, out=free), policy.linear(x, w, b))
+
+
+def test_collected_blocks_are_written_again(hip):
+    """collect reuses its blocks and writes the env's buffers: graphs that saved either are refused after the next call."""
+    from drone_amd.env import Drone
+
+    env = Drone(num_envs=300, device="cuda:0", seed=3, log_interval=0)
+    env.reset(3)
+    net = policy.Policy(width=32, device="cuda:0")
+    blocks = env.collect(net, 3)
+    versions = [b._version for b in blocks[:5]] + [v._version for v in (env.observations, env.actions, env.rewards, env.terminals, env.truncations)]
+    of_block, of_now = net(blocks[0]), net(env.observations)
+    env.collect(net, 3)
+    after = [b._version for b in blocks[:5]] + [v._version for v in (env.observations, env.actions, env.rewards, env.terminals, env.truncations)]
+    assert all(n > v for n, v in zip(after, versions))
+    for y in (of_block, of_now):
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    env.close()
+
+
+def test_out_that_autograd_knows_is_refused():
+    x, w = rand(6, 8, seed=1), rand(5, 8, seed=2)
+    leaf = torch.zeros(6, 5, device="cuda", requires_grad=True)
+    for out in (leaf, leaf * 2):
+        with pytest.raises(ValueError, match="out= cannot be differentiated"):
+            policy.linear(x, w, out=out)
+    with torch.no_grad():
+        policy.linear(x, w, out=leaf)
+    assert torch.equal(leaf, policy.linear(x, w))
