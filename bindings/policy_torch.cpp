@@ -7,6 +7,7 @@
 
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <cstring>
 #include <string>
@@ -62,6 +63,12 @@ void check(const char* name, const Tensor& t, at::IntArrayRef shape, const Tenso
     TORCH_CHECK_VALUE(t.sizes() == shape, name, " has shape ", t.sizes(), ", expected ", shape);
     TORCH_CHECK_TYPE(t.scalar_type() == x.scalar_type(), name, " is ", t.scalar_type(), ", x is ", x.scalar_type());
     TORCH_CHECK_VALUE(t.device() == x.device(), name, " is on ", t.device(), ", x on ", x.device());
+}
+
+// What would vanish without a word: a call that torch.jit traces (it would record the empty output), a dual tensor's tangent.
+void not_traced(const char* what) { TORCH_CHECK(!torch::jit::tracer::isTracing(), what, " cannot be traced"); }
+void no_tangent(const char* what, const Tensor& t) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), what, " has no forward-mode derivative");
 }
 
 bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
@@ -177,6 +184,8 @@ bool overlap(const Tensor& a, const Tensor& b) {
 
 Tensor linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, const std::string& activation, const OptTensor& residual, const OptTensor& out) {
     dtype_of(x, "x");
+    not_traced("linear");
+    for (const Tensor& t : {x, weight, bias.value_or(Tensor()), residual.value_or(Tensor()), out.value_or(Tensor())}) no_tangent("linear", t);
     const int act = activation_of(activation);
     TORCH_CHECK_VALUE(weight.dim() == 2 && x.dim() >= 1, "weight must be [out, in] and x [..., in], got ", weight.sizes(), " and ", x.sizes());
     const int64_t n = weight.size(0), k = weight.size(1);
@@ -283,6 +292,8 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
 
 std::tuple<Tensor, Tensor> norm_residual(const Tensor& x, const OptTensor& block, const OptTensor& gate, double scale, const OptTensor& post_weight, const OptTensor& pre_weight, double eps) {
     dtype_of(x, "x");
+    not_traced("norm_residual");
+    for (const Tensor& t : {x, block.value_or(Tensor()), gate.value_or(Tensor()), post_weight.value_or(Tensor()), pre_weight.value_or(Tensor())}) no_tangent("norm_residual", t);
     TORCH_CHECK_VALUE(x.dim() >= 1, "x must be [..., width]");
     const int64_t width = x.size(-1);
     TORCH_CHECK_VALUE(width >= 1 && width <= 4096, "width must be 1 ... 4096, got ", width);
@@ -316,6 +327,7 @@ std::tuple<Tensor, Tensor> norm_residual(const Tensor& x, const OptTensor& block
 Tensor adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& exp_avgs, const std::vector<Tensor>& exp_avg_sqs, const Tensor& step, double lr,
                   std::pair<double, double> betas, double eps, double weight_decay, std::optional<double> max_grad_norm, const std::optional<std::vector<Tensor>>& masters) {
     TORCH_CHECK_VALUE(!params.empty(), "no parameters");
+    not_traced("adamw_step");
     const Tensor& first = params[0];
     const int dtype = dtype_of(first, "params[0]");
     TORCH_CHECK_VALUE(masters.has_value() == (dtype != DRONE_F32), "16-bit params need float32 masters, float32 params have none");

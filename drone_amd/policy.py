@@ -38,7 +38,7 @@ def _native():
 
 
 def linear(x, weight, bias=None, activation="none", residual=None, out=None):
-    """``act(x @ weight.T + bias) + residual`` in one launch, differentiable (once) in all four.
+    """``act(x @ weight.T + bias) + residual`` in one launch, differentiable (once, backward) in all four.
 
     x ``[..., in]``, weight ``[out, in]``, bias ``[out]``, residual ``[..., out]``, one type (float32, bfloat16, float16)
     and one GPU; activation: none, relu, tanh, silu, gelu (the erf form). Sums are 32-bit, the result is rounded once; calls of
@@ -56,7 +56,8 @@ def norm_residual(x, block=None, *, gate=None, scale=1.0, post_weight=None, pre_
 
     ``r`` is the residual stream behind the block, ``h`` what the next block reads. x, block ``[..., width]``; gate
     ``[width]`` or ``[..., width]`` or None (1); weights ``[width]`` or None (1); width 1 ... 4096. Without a block
-    ``r = x``. Differentiable (once) in all five tensors; scale and eps are numbers."""
+    ``r = x``. Differentiable (once, backward) in all five tensors; scale and eps are
+    numbers."""
     return _native().norm_residual(x, block, gate, scale, post_weight, pre_weight, eps)
 
 

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from drone_amd import policy
-from test_policy_gpu import TYPES, check_norm, linear_case, norm_case, rand
+from test_policy_gpu import TYPES, adamw_case, check_norm, linear_case, norm_case, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -83,3 +83,40 @@ def test_out_that_autograd_knows_is_refused():
     with torch.no_grad():
         policy.linear(x, w, out=leaf)
     assert torch.equal(leaf, policy.linear(x, w))
+
+
+def test_forward_mode_and_tracing_are_refused():
+    """Neither has a formula here: a dual tensor's tangent, or a traced call, would vanish without a word."""
+    import torch.autograd.forward_ad as fwd
+
+    x, w, b, r, _ = (v.detach() for v in linear_case(6, 8, 5, torch.float32, "tanh"))
+    n = r.shape[1]
+    with fwd.dual_level():
+        for at in range(4):
+            for grad in (False, True):
+                a = [v.clone().requires_grad_(grad) for v in (x, w, b, r)]
+                a[at] = fwd.make_dual(a[at], torch.ones_like(a[at]))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    policy.linear(a[0], a[1], a[2], "tanh", a[3])
+        for at in range(5):
+            for grad in (False, True):
+                a = [v.clone().requires_grad_(grad) for v in (r, r, r, b, b)]
+                a[at] = fwd.make_dual(a[at], torch.ones_like(a[at]))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    policy.norm_residual(a[0], a[1], gate=a[2], post_weight=a[3], pre_weight=a[4])
+    assert n == 5
+    for f in (lambda v: policy.linear(v, w, b), lambda v: policy.norm_residual(v)[0], lambda v: policy.linear(v, w, b, out=torch.empty(6, 5, device="cuda"))):
+        with pytest.raises(RuntimeError, match="trac"):
+            torch.jit.trace(f, (x,), check_trace=False)
+    s = adamw_case([(4,)], torch.float32)
+
+    def traced(v):
+        policy.adamw_step(s["params"], s["grads"], s["m"], s["v"], s["step"], lr=1e-3)
+        return v + 1
+
+    with pytest.raises(RuntimeError, match="trac"):
+        torch.jit.trace(traced, (x,), check_trace=False)
+    for transform in (lambda: torch.func.jvp(lambda v: policy.linear(v, w, b), (x,), (x,)), lambda: torch.func.vmap(lambda v: policy.linear(v, w, b))(x.view(2, 3, 8)),
+                      lambda: torch.func.grad(lambda v: policy.linear(v, w, b).sum())(x)):
+        with pytest.raises(RuntimeError):
+            transform()
