@@ -4,9 +4,9 @@
 //   p = p (1 - lr wd) - lr (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps)
 // Two launches whatever the number of tensors (up to kAdamwTensors): the norm's partial sums (and the step counter, in HBM
 // so that a captured step replays with an advancing t), then the update; one launch of one workgroup where all the tensors
-// together are a few chunks (the six tensors of a 20-64-64-4 policy: 7.8 us, 9.6 in two). Everything in 32 bits; a 16-bit weight is its 32-bit master rounded once, and the master is what
-// the next step starts from. Bound by memory: 21e6 16-bit weights with masters, 630 MB, 23 + 105 us (4.9 TB/s; a copy reaches
-// 5.1; the norm has to have read every gradient before the first update, and reads them from the cache's leavings again).
+// together are a few chunks (the six tensors of a 20-64-64-4 policy: 7.8 us, 9.6 in two). Everything in 32 bits; a 16-bit
+// weight is its 32-bit master rounded once, and the master is what the next step starts from unless the weight is no longer
+// that. Bound by memory: 21e6 16-bit weights with masters, 672 MB, 135 us (5.0 TB/s; a copy reaches 5.1; the norm has to have read every gradient before the first update, and reads them from the cache's leavings again).
 #include <hip/hip_runtime.h>
 
 #include "drone_policy.hpp"
@@ -100,7 +100,15 @@ struct Eight {
         load8((const T*)t.g, i, t.n, t.vec, g);
         load8(t.m, i, t.n, t.vec, m);
         load8(t.v, i, t.n, t.vec, v);
-        if (t.master) load8(t.master, i, t.n, t.vec, p); else load8((const T*)t.p, i, t.n, t.vec, p);
+        load8((const T*)t.p, i, t.n, t.vec, p);
+        if (sizeof(T) == 4) return;
+        // A 16-bit weight that is not its rounded master has been written since the last step (a loaded state, a target's
+        // copy): the step starts from it. The two bytes more cost 21e6
+        // weights 8 us (135 against 127).
+        float master[8];
+        load8(t.master, i, t.n, t.vec, master);
+#pragma unroll
+        for (int k = 0; k < 8; k++) p[k] = (float)(T)master[k] == p[k] ? master[k] : p[k];
     }
     __device__ __forceinline__ void step(const AdamwArgs& a, const Step& s) {
 #pragma unroll
@@ -114,7 +122,7 @@ struct Eight {
     __device__ __forceinline__ void store(const AdamwTensor& t, long long i) const {
         store8(t.m, i, t.n, t.vec, m);
         store8(t.v, i, t.n, t.vec, v);
-        if (t.master) store8(t.master, i, t.n, t.vec, p);
+        if (sizeof(T) == 2) store8(t.master, i, t.n, t.vec, p);
         store8((T*)t.p, i, t.n, t.vec, p);
     }
 };

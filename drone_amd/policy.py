@@ -68,7 +68,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.
     (``[1]`` float32 on the device). ``max_grad_norm``: scale the gradients by ``min(1, max_grad_norm / (norm + 1e-6))``.
 
     params and grads of one type; exp_avgs, exp_avg_sqs float32; 16-bit params need float32 ``masters`` (the params are
-    their rounded copies). ``step``: int32 tensor ``[1]`` on the device, the steps done so far; the call adds 1, so a step
+    their rounded copies; a value that is not has been written since, and the step starts from it). ``step``: int32 tensor ``[1]`` on the device, the steps done so far; the call adds 1, so a step
     captured into a graph replays with an advancing count. All tensors contiguous, on one GPU, none twice."""
     return _native().adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas, eps, weight_decay, max_grad_norm, masters)
 
@@ -84,7 +84,8 @@ def _check_parameter(p):
 
 class AdamW(torch.optim.Optimizer):
     """``adamw_step`` as a torch optimizer: one parameter group's tensors of one type per step call, moments and (for 16-bit
-    parameters) masters in float32. ``max_grad_norm`` clips by the norm over a whole group; ``grad_norm`` holds the last
+    parameters) masters in float32. Weights may be written between steps (a loaded state, a target network's copy): the next
+    step starts from what is there. ``max_grad_norm`` clips by the norm over a whole group; ``grad_norm`` holds the last
     step's norms, one ``[1]`` tensor per group. Parameters without a gradient are left alone; the step count is the
     group's. ``lr`` and the rest are read at every call (a captured step keeps those of its capture)."""
 

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from drone_amd import policy
-from test_policy_gpu import TYPES, adamw_case, check_norm, linear_case, norm_case, rand
+from test_policy_gpu import MLP, TYPES, adamw_case, check_norm, half_step, linear_case, norm_case, rand, step
 
 pytestmark = pytest.mark.gpu
 
@@ -120,3 +120,59 @@ def test_forward_mode_and_tracing_are_refused():
                       lambda: torch.func.grad(lambda v: policy.linear(v, w, b).sum())(x)):
         with pytest.raises(RuntimeError):
             transform()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("shapes", [MLP, [(300, 257), (129, 513), (5,)]])
+def test_weights_written_between_steps_are_kept(t, shapes):
+    """A weight written after the optimizer was built (a loaded state, a re-initialised layer, a target network's copy) is
+    what the next step starts from, one element or all of them; the untouched ones keep their 32-bit masters."""
+    ps = [torch.nn.Parameter(rand(*d, to=t, seed=i)) for i, d in enumerate(shapes)]
+    opt = policy.AdamW(ps, lr=1e-2, weight_decay=0.0)
+    for k, p in enumerate(ps):
+        p.grad = rand(*p.shape, to=t, of=0.1, seed=50 + k)
+    opt.step()
+    masters = [(opt.state[p]["master"] if t != torch.float32 else p.detach()).clone() for p in ps]
+    with torch.no_grad():
+        ps[0].copy_(rand(*ps[0].shape, to=t, seed=90))
+        ps[1][1] = -3.0
+    # (a written value that the master rounds to cannot be told from the old one: the master is it, to the type's precision)
+    starts = [torch.where(masters[0].to(t) == ps[0], masters[0], ps[0].float()).detach(), masters[1].clone(), *masters[2:]]
+    starts[1][1] = -3.0
+    twins = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    other = policy.AdamW(twins, lr=1e-2, weight_decay=0.0)
+    other.load_state_dict(opt.state_dict())
+    for p, q, s in zip(ps, twins, starts):
+        q.grad = p.grad
+        if t != torch.float32:
+            other.state[q]["master"].copy_(s)
+    opt.step()
+    other.step()
+    for p, q in zip(ps, twins):
+        assert torch.equal(p, q)
+        if t != torch.float32:
+            assert torch.equal(opt.state[p]["master"], other.state[q]["master"]) and torch.equal(p, opt.state[p]["master"].to(t))
+    assert (ps[0].detach().float() - starts[0]).abs().max().item() <= 1.1e-2 + half_step(t) * 5  # a step of lr, and its rounding
+
+
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16])
+def test_weights_written_between_replays_are_kept(t):
+    """The same for a captured step, which no Python runs before."""
+    p = torch.nn.Parameter(rand(40, 30, to=t, seed=1))
+    p.grad = rand(40, 30, to=t, seed=2)
+    opt = policy.AdamW([p], lr=1e-3, weight_decay=0.0)
+    opt.step()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        opt.step()
+    for k in range(3):
+        loaded = rand(40, 30, to=t, seed=10 + k)
+        with torch.no_grad():
+            p.copy_(loaded)
+        g.replay()
+        torch.cuda.synchronize()
+        # a step of lr, from a start that is the loaded value or rounds to it: within half a step of the type of it
+        over = (opt.state[p]["master"].double() - loaded.double()).abs() - 1.1e-3 - half_step(t) * loaded.double().abs()
+        assert over.max().item() <= 0 and torch.equal(p, opt.state[p]["master"].to(t))
+        assert not torch.equal(opt.state[p]["master"], loaded.float())
+    assert opt.param_groups[0]["step"].item() == 4
