@@ -14,6 +14,7 @@
 // Odd widths take the streaming gradients too, on operands laid out in whole pieces (linear_dz_kernel, linear_pad_kernel).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "drone_policy.hpp"
@@ -25,6 +26,7 @@ namespace {
 
 constexpr int kPieces = 8;  // 16-byte pieces of the reduction axis a tile row holds: 64 16-bit or 32 f32 elements
 constexpr int kJoinThreads = 256;
+constexpr long long kJoinBlocks = 1 << 22;  // of the join at most: a launch of 2^32 threads or more runs only some of them, without an error
 
 template <class T> __device__ __forceinline__ float to_f(T v) { return (float)v; }
 
@@ -1148,21 +1150,26 @@ template <class T>
 __global__ __launch_bounds__(kJoinThreads) void linear_join_kernel(const float* work, const float* db_work, T* dw, T* db, long long weights, int out, int w_parts, int b_parts) {
     __shared__ float join[8][32];
     const int c = threadIdx.x & 31, slice = threadIdx.x >> 5;
-    const long long i = (long long)blockIdx.x * 32 + c, nw = dw ? weights : 0, all = nw + (db ? out : 0);
-    const bool is_w = i < nw;
-    const long long at = is_w ? i : i - nw, step = is_w ? weights : out;
-    const float* p = (is_w ? work : db_work) + at;
-    const int parts = is_w ? w_parts : b_parts;
-    float s = 0.f;
-    if (i < all)
+    const long long nw = dw ? weights : 0, all = nw + (db ? out : 0);
+    for (long long first = (long long)blockIdx.x * 32; first < all; first += (long long)gridDim.x * 32) {  // (once, up to kJoinBlocks)
+        const long long i = first + c;
+        const bool is_w = i < nw;
+        const long long at = is_w ? i : i - nw, step = is_w ? weights : out;
+        const float* p = (is_w ? work : db_work) + at;
+        const int parts = is_w ? w_parts : b_parts;
+        float s = 0.f;
+        if (i < all)
 #pragma unroll 4
-        for (int k = slice; k < parts; k += 8) s += p[k * step];
-    join[slice][c] = s;
-    __syncthreads();
-    if (slice || i >= all) return;
+            for (int k = slice; k < parts; k += 8) s += p[k * step];
+        join[slice][c] = s;
+        __syncthreads();
+        if (!slice && i < all) {
 #pragma unroll
-    for (int k = 1; k < 8; k++) s += join[k][c];
-    if (is_w) dw[at] = (T)s; else db[at] = (T)s;
+            for (int k = 1; k < 8; k++) s += join[k][c];
+            if (is_w) dw[at] = (T)s; else db[at] = (T)s;
+        }
+        __syncthreads();
+    }
 }
 
 template <class T, Product P, int BM, int BN, int WM, int WN>
@@ -1421,7 +1428,7 @@ int backward_any(LinearArgs a, hipStream_t s) {
     }
     if (rc) return rc;
     const long long weights = (long long)a.out * a.in, all = (a.dw ? weights : 0) + (a.db ? a.out : 0);
-    linear_join_kernel<T><<<(unsigned)((all + 31) / 32), kJoinThreads, 0, s>>>(dw_work, db_work, (T*)a.dw, (T*)a.db, weights, a.out, p.w_parts, p.db_parts);
+    linear_join_kernel<T><<<(unsigned)std::min((all + 31) / 32, kJoinBlocks), kJoinThreads, 0, s>>>(dw_work, db_work, (T*)a.dw, (T*)a.db, weights, a.out, p.w_parts, p.db_parts);
     return (int)hipGetLastError();
 }
 

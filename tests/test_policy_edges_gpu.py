@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from drone_amd import policy
-from test_policy_gpu import MLP, TYPES, adamw_case, check_norm, half_step, linear_case, norm_case, rand, step
+from test_policy_gpu import MLP, TINY, TYPES, U32, adamw_case, check_norm, close, half_step, linear_case, norm_case, rand, step
 
 pytestmark = pytest.mark.gpu
 
@@ -176,3 +176,17 @@ def test_weights_written_between_replays_are_kept(t):
         assert over.max().item() <= 0 and torch.equal(p, opt.state[p]["master"].to(t))
         assert not torch.equal(opt.state[p]["master"], loaded.float())
     assert opt.param_groups[0]["step"].item() == 4
+
+
+@pytest.mark.parametrize("t", [torch.bfloat16])
+def test_linear_weight_gradient_of_a_very_wide_layer(t):
+    """2^29 weights: more joins than one launch has threads for."""
+    n, k = 32768, 16384
+    x, dy = rand(2, k, to=t, seed=1), rand(2, n, to=t, seed=2)
+    w = torch.zeros(n, k, dtype=t, device="cuda").requires_grad_(True)
+    b = torch.zeros(n, dtype=t, device="cuda").requires_grad_(True)
+    dw, db = torch.autograd.grad(policy.linear(x, w, b), [w, b], dy)
+    close(db, dy.double().sum(0), dy.double().abs().sum(0) * (half_step(t) + 2 * U32) + TINY[t], "db")
+    for at in range(0, n, 4096):
+        d = dy[:, at:at + 4096].double()
+        close(dw[at:at + 4096], d.t() @ x.double(), d.abs().t() @ x.double().abs() * (half_step(t) + 4 * U32) + TINY[t], f"dw {at}")
