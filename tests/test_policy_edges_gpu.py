@@ -178,6 +178,27 @@ def test_weights_written_between_replays_are_kept(t):
     assert opt.param_groups[0]["step"].item() == 4
 
 
+def diagonal(m, n, t, z):
+    """A layer whose z is its x: the unit weight, no bias; the rows hold the values of z in turn."""
+    x = z[torch.arange(m * n, device="cuda") % z.numel()].view(m, n).to(t)
+    return x.requires_grad_(True), torch.eye(n, device="cuda").to(t).requires_grad_(True)
+
+
+FORMS = [(5, 64), (333, 65), (5000, 64), (9001, 100), (66001, 256), (20001, 333)]  # few rows, tiled, one pass, odd widths, streamed
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m, n", FORMS + [(270001, 64)])
+def test_linear_tanh_near_zero(t, m, n):
+    """tanh of small z, relative to itself: the rounding to the type and 2e-6 (a dozen 32-bit operations)."""
+    z = torch.logspace(-8, -0.5, 41, device="cuda")
+    x, w = diagonal(m, n, t, torch.cat([z, -z]))
+    with torch.no_grad():
+        y = policy.linear(x, w, None, "tanh")
+    want = torch.tanh(x.detach().double())
+    close(y, want, want.abs() * (half_step(t) + 2e-6) + TINY[t], f"{m}x{n}")
+
+
 @pytest.mark.parametrize("t", [torch.bfloat16])
 def test_linear_weight_gradient_of_a_very_wide_layer(t):
     """2^29 weights: more joins than one launch has threads for."""
