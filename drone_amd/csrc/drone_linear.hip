@@ -32,7 +32,7 @@ template <class T> __device__ __forceinline__ float to_f(T v) { return (float)v;
 
 // ---- activation: value and slope in 32 bits, by the hardware's exp2 and rcp (1 ulp each). f32 tensors: tanh by its series
 // near zero and erf from the math library. 16-bit tensors: the instructions count (the epilogue of a narrow layer is as long as
-// its product): tanh = 1 - 2 / (1 + exp 2z), 2e-6 of itself off at most, and below 0.1 (where that would lose 1e-7 / z) two
+// its product): |tanh| = 1 - 2 / (1 + exp 2|z|), 2e-6 of itself off at most, and below 0.1 (where that would lose 1e-7 / z) two
 // terms of the series; erfc by Abramowitz & Stegun 7.1.26 (|error| <= 1.5e-7; relative to gelu 5e-5 at z = -3, 5e-4 at -4,
 // 4e-3 at -6, where it is 6e-9), whose exp(-z^2/2) is also what the slope needs. The forms are chosen so that infinities give
 // the limits (no 0 * inf) and NaNs stay. ----
@@ -51,9 +51,9 @@ __device__ __forceinline__ float activate(float z, float& slope) {
                 slope = small ? 1.f - series * series : x * (2.f - x);
                 return small ? series : copysignf(1.f - x, z);
             }
-            const float r = __builtin_amdgcn_rcpf(1.f + __expf(2.f * z)), q = z * z;
+            const float r = __builtin_amdgcn_rcpf(1.f + __expf(2.f * fabsf(z))), q = z * z;  // r: (1 - |tanh z|) / 2
             slope = 4.f * r * (1.f - r);
-            return q < 0.01f ? z * (1.f + q * (-0.33333334f + q * 0.13333334f)) : 1.f - 2.f * r;  // (next term: 5e-8 of z)
+            return q < 0.01f ? z * (1.f + q * (-0.33333334f + q * 0.13333334f)) : copysignf(1.f - 2.f * r, z);  // (next term: 5e-8 of z)
         }
         case DRONE_ACTIVATION_SILU: {
             const float s = __builtin_amdgcn_rcpf(1.f + __expf(-z)), c = fminf(fmaxf(z, -90.f), 90.f);

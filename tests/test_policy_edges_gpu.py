@@ -211,3 +211,25 @@ def test_linear_weight_gradient_of_a_very_wide_layer(t):
     for at in range(0, n, 4096):
         d = dy[:, at:at + 4096].double()
         close(dw[at:at + 4096], d.t() @ x.double(), d.abs().t() @ x.double().abs() * (half_step(t) + 4 * U32) + TINY[t], f"dw {at}")
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.float16])
+@pytest.mark.parametrize("act", ["tanh", "silu"])
+@pytest.mark.parametrize("m, n", FORMS)
+def test_linear_gradient_of_saturated_units(t, act, m, n):
+    """The slopes of far z, relative to themselves: 1e-5 for the exponential
+    of an argument up to 20 (rounded to 2^-24 of itself) and a handful of operations on it, and the roundings of dz and dx to
+    the type. (dx is dz times one.) dy is a power of two large enough that dz is a normal number of the type."""
+    z = torch.arange(-20, 21, device="cuda") / 2.0
+    z = z[z.abs() >= 2.5]
+    z = z[z < 0] if act == "silu" else z  # (silu's slope is near 1 on the other side)
+    if t == torch.float16:
+        z = z[z.abs() <= 8]
+    x, w = diagonal(m, n, t, z)
+    dy = torch.full((m, n), 2.0 ** 12, device="cuda").to(t)
+    dx, _ = torch.autograd.grad(policy.linear(x, w, None, act), [x, w], dy)
+    Z = x.detach().double()
+    s = 1 / torch.cosh(Z).square() if act == "tanh" else torch.sigmoid(Z) * (1 + Z * torch.sigmoid(-Z))
+    want = 2.0 ** 12 * s
+    tol = want.abs() * (2 * half_step(t) + 1e-5)
+    close(dx, want, tol, f"{act} {m}x{n}")
