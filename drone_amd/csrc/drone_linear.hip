@@ -29,6 +29,7 @@ constexpr int kJoinThreads = 256;
 constexpr long long kJoinBlocks = 1 << 22;  // of the join at most: a launch of 2^32 threads or more runs only some of them, without an error
 
 template <class T> __device__ __forceinline__ float to_f(T v) { return (float)v; }
+template <class T> __device__ __forceinline__ float to_slope(typename Elem<T>::Slope v) { return (float)v * (1.f / Elem<T>::kSlopeScale); }
 
 // ---- activation: value and slope in 32 bits, by the hardware's exp2 and rcp (1 ulp each). f32 tensors: tanh by its series
 // near zero and erf from the math library. 16-bit tensors: the instructions count (the epilogue of a narrow layer is as long as
@@ -184,7 +185,7 @@ struct ContigTile {
                 using S = typename Elem<T>::Slope;
                 const auto q = WHOLE ? load_n<S, kE>(o.slope + r * o.slope_ld + k, kE) : load_end<S, kE>(o.slope + r * o.slope_ld, k, kend);
 #pragma unroll
-                for (int e = 0; e < kE; e++) reg[i].e[e] = (T)(to_f(reg[i].e[e]) * to_f(q.e[e]));
+                for (int e = 0; e < kE; e++) reg[i].e[e] = (T)(to_f(reg[i].e[e]) * to_slope<T>(q.e[e]));
             }
         }
     }
@@ -230,7 +231,7 @@ struct TransTile {
                 if (o.slope) {
                     const auto q = WHOLE ? load_n<S, 4>(o.slope + at * o.slope_ld + r, 4) : load_end<S, 4>(o.slope + at * o.slope_ld, r, rows);
 #pragma unroll
-                    for (int j = 0; j < 4; j++) { f[j] *= to_f(q.e[j]); v.e[j] = (T)f[j]; }
+                    for (int j = 0; j < 4; j++) { f[j] *= to_slope<T>(q.e[j]); v.e[j] = (T)f[j]; }
                 }
                 if (!WHOLE)
 #pragma unroll
@@ -333,7 +334,7 @@ __device__ __forceinline__ void write_forward(const LinearArgs& a, const f32x16 
                 float v[kE], s[kE];
                 const Piece bias = __builtin_bit_cast(Piece, b[n][q]);
 #pragma unroll
-                for (int j = 0; j < kE; j++) v[j] = activate<ACT, sizeof(T) == 4>(acc[n][m][kE * q + j] + to_f(bias.e[j]), s[j]);
+                for (int j = 0; j < kE; j++) { v[j] = activate<ACT, sizeof(T) == 4>(acc[n][m][kE * q + j] + to_f(bias.e[j]), s[j]); s[j] *= Elem<T>::kSlopeScale; }
                 if (a.slope) store_n<Slope, kE>((Slope*)a.slope + row * a.out + feat, left, s);
                 if (a.res) {
                     const Piece r = __builtin_bit_cast(Piece, res[m][n][q]);
@@ -762,7 +763,7 @@ __device__ __forceinline__ void resident_forward(const LinearArgs& a, u32x4 (*ld
                 if (n <= 0) continue;
                 float v[kE], s[kE];
 #pragma unroll
-                for (int j = 0; j < kE; j++) v[j] = activate<ACT, sizeof(T) == 4>(acc[q * kE + j], s[j]);
+                for (int j = 0; j < kE; j++) { v[j] = activate<ACT, sizeof(T) == 4>(acc[q * kE + j], s[j]); s[j] *= Elem<T>::kSlopeScale; }
                 if (SLOPE) store_n<Slope, kE>((Slope*)a.slope + row * a.out + column(q), n, s);
                 if (RES) {
                     const auto more = __builtin_bit_cast(Vec<T, kE>, lds[buf][M::kX + M::R::at(r, (column(q) - group0) / kE)]);
@@ -815,7 +816,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(LinearArgs a, T* dz, lon
             if (a.slope) {
                 const auto q = WHOLE ? load_n<Slope, kE>((const Slope*)a.slope + r * a.out + col, kE) : load_end<Slope, kE>((const Slope*)a.slope + r * a.out, col, a.out);
 #pragma unroll
-                for (int e = 0; e < kE; e++) f[e] *= to_f(q.e[e]);
+                for (int e = 0; e < kE; e++) f[e] *= to_slope<T>(q.e[e]);
             }
             if (dz) store_n<T, kE>(dz + r * dz_ld + col, kE, f);
 #pragma unroll
@@ -998,7 +999,7 @@ __global__ __launch_bounds__(kBackThreads, 2) void linear_back_kernel(LinearArgs
                 for (int k = 0; k < kPer; k++) {
                     const auto q = __builtin_bit_cast(SlopePiece, t[M::kS + M::S::at(r, piece * kPer + k)]);
 #pragma unroll
-                    for (int e = 0; e < kSE; e++) f[k * kSE + e] *= to_f(q.e[e]);
+                    for (int e = 0; e < kSE; e++) f[k * kSE + e] *= to_slope<T>(q.e[e]);
                 }
             }
             if (last && row0 + r >= a.rows)
@@ -1096,7 +1097,7 @@ __device__ __forceinline__ void few_forward(const LinearArgs& a, const float* su
 #pragma unroll
         for (int w = 0; w < 8; w++) z += sums[w * 1024 + r * 32 + f + j];
         float v = activate<ACT, sizeof(T) == 4>(z, s);
-        if (a.slope) ((typename Elem<T>::Slope*)a.slope)[row * a.out + feat] = (typename Elem<T>::Slope)s;
+        if (a.slope) ((typename Elem<T>::Slope*)a.slope)[row * a.out + feat] = (typename Elem<T>::Slope)(s * Elem<T>::kSlopeScale);
         if (a.res) v += to_f(((const T*)a.res)[row * a.res_ld + feat]);
         ((T*)a.y)[row * a.y_ld + feat] = (T)v;
     }

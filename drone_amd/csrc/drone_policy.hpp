@@ -110,12 +110,14 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 // kE elements make a 16-byte piece; Slope: the type act'(z) is kept in between forward and backward, finer than T, so that a
-// 16-bit layer's gradient carries only the two roundings nobody can avoid (dz into the matrix core, the result into memory).
-// A slope lies in [-0.13, 1.13], where fp16 has eight times bf16's steps at the same size; fp16 itself needs f32.
+// 16-bit layer's gradient carries only two roundings (dz into the matrix core, the result into memory). A bf16 layer's are fp16
+// times kSlopeScale: slopes lie in [-0.13, 1.13], so the products stay below 37 100, and a saturated unit's slope keeps eleven
+// bits down to 2^-29 (tanh: |z| = 10.7; without the scale 5.5, and nothing left from 10 on) and bf16's eight to 2^-32. fp16
+// itself needs f32.
 template <class T> struct Elem;
-template <> struct Elem<float> { static constexpr int kE = 4; using Slope = float; };
-template <> struct Elem<__bf16> { static constexpr int kE = 8; using Slope = _Float16; };
-template <> struct Elem<_Float16> { static constexpr int kE = 8; using Slope = float; };
+template <> struct Elem<float> { static constexpr int kE = 4; using Slope = float; static constexpr float kSlopeScale = 1.f; };
+template <> struct Elem<__bf16> { static constexpr int kE = 8; using Slope = _Float16; static constexpr float kSlopeScale = 32768.f; };
+template <> struct Elem<_Float16> { static constexpr int kE = 8; using Slope = float; static constexpr float kSlopeScale = 1.f; };
 
 }  // namespace drone
 #endif

@@ -378,9 +378,9 @@ int drone_vec_copy_to_host(DroneVec* v, void* host_dst, const void* device_src, 
 
 /* y = act(x W^T + b) + residual: one launch. x [rows][in], weight [out][in], bias [out], residual / y [rows][out], all of
  * `dtype`; products are summed in 32 bits, the result is rounded once. `slope` (forward, or NULL when nothing will be
- * differentiated) receives act'(z), [rows][out] dense, fp16 for DRONE_BF16 and f32 for the others. Backward reads it
- * (NULL only for DRONE_ACTIVATION_NONE) with dy [rows][out] and writes those of
- *   dx = dz W,   dweight = dz^T x,   dbias = sum of dz over the rows,   dz = dy * slope
+ * differentiated) receives act'(z) for the backward call, [rows][out] dense: f32, for DRONE_BF16 2^15 act'(z) in fp16.
+ * Backward reads it (NULL only for DRONE_ACTIVATION_NONE) with dy [rows][out] and writes those of
+ *   dx = dz W,   dweight = dz^T x,   dbias = sum of dz over the rows,   dz = dy act'(z)
  * that are not NULL (dweight [out][in] and dbias [out] dense); the residual's gradient is dy itself. y may be the residual
  * (same pointer and leading dimension); no other output may overlap an input. rows 0 ... 2^30 (0: sums are zero),
  * in / out 1 ... 65536. Backward with dweight or dbias needs drone_linear_workspace bytes at `workspace` (16-byte aligned):
