@@ -92,6 +92,13 @@ __global__ __launch_bounds__(kThreads) void adamw_norm_kernel(AdamwArgs a) {
 // units busy for 7 us of a 5 764-weight step.
 struct Step { float clip, rate, unbias; };
 
+// The hardware's square root takes a denormal number for 0: v of gradients around 1e-19 is scaled into the normal ones and back.
+// (Its reciprocal does so too, but eps is normal, and what is added to it no less.)
+__device__ __forceinline__ float root(float v) {
+    const bool low = v < 0x1p-96f;
+    return __builtin_amdgcn_sqrtf(low ? v * 0x1p64f : v) * (low ? 0x1p-32f : 1.f);
+}
+
 // Eight elements and their state: asked for in one go, updated, stored.
 template <class T>
 struct Eight {
@@ -116,7 +123,7 @@ struct Eight {
             const float d = g[k] * s.clip;
             m[k] = a.b1 * m[k] + a.rest1 * d;
             v[k] = a.b2 * v[k] + a.rest2 * d * d;
-            p[k] = p[k] * a.decay - s.rate * m[k] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[k] * s.unbias) + a.eps);
+            p[k] = p[k] * a.decay - s.rate * m[k] * __builtin_amdgcn_rcpf(root(v[k] * s.unbias) + a.eps);
         }
     }
     __device__ __forceinline__ void store(const AdamwTensor& t, long long i) const {

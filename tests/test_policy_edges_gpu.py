@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from drone_amd import policy
-from test_policy_gpu import MLP, TINY, TYPES, U32, adamw_case, check_norm, close, half_step, linear_case, norm_case, rand, step
+from test_policy_gpu import HYPER, MLP, TINY, TYPES, U32, adamw_case, check_norm, close, half_step, linear_case, norm_case, rand, step
 
 pytestmark = pytest.mark.gpu
 
@@ -197,6 +197,22 @@ def test_linear_tanh_near_zero(t, m, n):
         y = policy.linear(x, w, None, "tanh")
     want = torch.tanh(x.detach().double())
     close(y, want, want.abs() * (half_step(t) + 2e-6) + TINY[t], f"{m}x{n}")
+
+
+@pytest.mark.parametrize("shapes", [MLP, [(300, 257), (129, 513)]])
+def test_adamw_of_denormal_moments(shapes):
+    """Gradients of 1e-20 and an eps below them: v is a denormal number and counts all the same. Against the formula on the
+    moments as they were stored: a few 2^-24 of the step, and half a step of a denormal v / (1 - b2^t) around 1e-40 (2e-5)."""
+    s = adamw_case(shapes, torch.float32, zero=True)
+    for g in s["grads"]:
+        g.copy_(torch.where(g >= 0, 1e-20, -1e-20))
+    before = [p.double() for p in s["masters"]]
+    step(s, eps=1e-30, weight_decay=0.0)
+    (b1, b2), lr = HYPER["betas"], HYPER["lr"]
+    for p, q, m, v in zip(s["masters"], before, s["m"], s["v"]):
+        assert 0 < v.max().item() < 2.0 ** -126
+        move = lr * (m.double() / (1 - b1)) / (torch.sqrt(v.double() / (1 - b2)) + 1e-30)
+        close(p, q - move, 1e-4 * move.abs() + 2 * U32 * q.abs(), "p")
 
 
 @pytest.mark.parametrize("t", [torch.bfloat16])
