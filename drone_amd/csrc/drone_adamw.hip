@@ -75,16 +75,18 @@ __global__ __launch_bounds__(kThreads) void adamw_norm_kernel(AdamwArgs a) {
         if (a.norm && !a.chunks) *a.norm = 0.f;  // no gradients at all
     }
     if (!a.parts) return;
-    float sum = 0.f;
+    double sum = 0;  // a thread of the largest calls adds up 131 072 squares: in 32 bits equal ones were rounded alike, 9e-6 off at 2 048
     for (int chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
         const AdamwTensor& t = a.t[tensor_of(a, chunk)];
         float g[8];
         load8((const T*)t.g, (long long)(chunk - t.first_chunk) * kAdamwChunk + threadIdx.x * 8, t.n, t.vec, g);
+        float eight = 0.f;
 #pragma unroll
-        for (int k = 0; k < 8; k++) sum += g[k] * g[k];
+        for (int k = 0; k < 8; k++) eight += g[k] * g[k];
+        sum += eight;
     }
-    sum = block_sum(sum, join);
-    if (threadIdx.x == 0) a.partial[2 + a.part0 + blockIdx.x] = sum;
+    const float all = block_sum((float)sum, join);
+    if (threadIdx.x == 0) a.partial[2 + a.part0 + blockIdx.x] = all;
 }
 
 // What an element's update needs besides its own values: the clip, lr / (1 - b1^t) and 1 / (1 - b2^t). The update's square

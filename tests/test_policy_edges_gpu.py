@@ -1,5 +1,7 @@
 """The policy operators at the edges of what they allow: calls that the other tests do not make, each against 64-bit
 formulas, against the same work done another way, or refused."""
+import math
+
 import pytest
 import torch
 
@@ -227,6 +229,15 @@ def test_linear_weight_gradient_of_a_very_wide_layer(t):
     for at in range(0, n, 4096):
         d = dy[:, at:at + 4096].double()
         close(dw[at:at + 4096], d.t() @ x.double(), d.abs().t() @ x.double().abs() * (half_step(t) + 4 * U32) + TINY[t], f"dw {at}")
+
+
+def test_adamw_norm_of_many_equal_gradients():
+    """2^28 equal values, whose squares a running 32-bit sum takes in with the same rounding again and again."""
+    n = 1 << 28
+    s = {k: torch.full((n,), v, device="cuda") for k, v in (("p", 0.5), ("g", 0.1), ("m", 0.0), ("v", 0.0))}
+    norm = policy.adamw_step([s["p"]], [s["g"]], [s["m"]], [s["v"]], torch.zeros(1, dtype=torch.int32, device="cuda"), lr=1e-3, max_grad_norm=1.0)
+    want = s["g"][0].double().item() * math.sqrt(n)
+    assert abs(norm.item() - want) <= 64 * U32 * want
 
 
 @pytest.mark.parametrize("t", TYPES)
