@@ -86,6 +86,14 @@ __device__ __forceinline__ float row_sum(float v, float* join) {
 
 __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
 
+// sigmoid(z) and 1 - sigmoid(z), each to a few units of its own last place: the gate's gradient is their product, and 1 - s of a
+// wide open gate would cancel.
+__device__ __forceinline__ void sigmoids(float z, float& s, float& rest) {
+    const float e = __expf(-fabsf(z)), more = __builtin_amdgcn_rcpf(1.f + e), less = e * more;
+    s = z < 0.f ? less : more;
+    rest = z < 0.f ? more : less;
+}
+
 template <class T, int TPR, int NP, bool VEC>
 __global__ __launch_bounds__(kThreads) void norm_forward_kernel(NormArgs a) {
     constexpr int kE = Elem<T>::kE, kRows = kThreads / TPR;
@@ -217,7 +225,7 @@ __global__ __launch_bounds__(kThreads) void norm_backward_kernel(NormArgs a) {
         const int width = row < a.rows ? a.width : 0;
         // 1 / rms of the row; 0 behind the last one, whose zeros may add nothing to the column sums (without eps: 0 * inf)
         auto inverse = [&](float squares) { return width ? 1.f / sqrtf(squares * inv_width + a.eps) : 0.f; };
-        float r[NP][kE], nb[NP][kE], s[NP][kE], dh[NP][kE], d_[NP][kE], f[kE], sum = 0.f;
+        float r[NP][kE], nb[NP][kE], s[NP][kE], rest[NP][kE], dh[NP][kE], d_[NP][kE], f[kE], sum = 0.f;
 #pragma unroll
         for (int i = 0; i < NP; i++) {
             unpack<T>(x_[i], r[i]);
@@ -229,7 +237,7 @@ __global__ __launch_bounds__(kThreads) void norm_backward_kernel(NormArgs a) {
 #pragma unroll
             for (int e = 0; e < kE; e++) {
                 sum += nb[i][e] * nb[i][e];
-                s[i][e] = a.gate_rows ? sigmoid(s[i][e]) : 1.f;
+                if (a.gate_rows) sigmoids(s[i][e], s[i][e], rest[i][e]); else { s[i][e] = 1.f; rest[i][e] = 0.f; }
             }
         }
         if (row0 + step < a.rows) ask(row + step);
@@ -278,7 +286,7 @@ __global__ __launch_bounds__(kThreads) void norm_backward_kernel(NormArgs a) {
             for (int e = 0; e < kE; e++) {
                 const float td = r[i][e] * a.scale, u = td * s[i][e], w = a.post ? fq[e] : 1.f;
                 post_sum[i][e] += u * nb[i][e];
-                const float dg = u * (nb[i][e] * w) * (1.f - s[i][e]);
+                const float dg = u * (nb[i][e] * w) * rest[i][e];
                 gate_sum[i][e] += dg;
                 d[e] = dg;
                 r[i][e] = u * w;

@@ -231,6 +231,24 @@ def test_linear_weight_gradient_of_a_very_wide_layer(t):
         close(dw[at:at + 4096], d.t() @ x.double(), d.abs().t() @ x.double().abs() * (half_step(t) + 4 * U32) + TINY[t], f"dw {at}")
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("gate", ["channel", "full"])
+@pytest.mark.parametrize("m, c", [(33, 32), (50, 200), (9, 1500)])
+def test_norm_gate_gradient_of_open_and_shut_gates(t, gate, m, c):
+    """dgate carries s (1 - s): at a gate of 5 ... 14 both factors keep their own precision, 1e-5 for an exponential of an
+    argument up to 14 and the operations around it. dr alone, so that the other factors are one product each."""
+    (x, block, _, post, pre), dr, _ = norm_case(m, c, t, "none", leaf=False)
+    g = (torch.arange(m * c, device="cuda") % 10 + 5.0).view(m, c) * torch.where(torch.arange(c, device="cuda") % 2 == 0, 1.0, -1.0)
+    g = (g if gate == "full" else g[0]).to(t).requires_grad_(True)
+    dr = dr * 256
+    r, _ = policy.norm_residual(x, block, gate=g, scale=0.5, post_weight=post, pre_weight=pre)
+    got, = torch.autograd.grad(r, g, dr)
+    B, G = block.double(), g.detach().double()
+    each = dr.double() * 0.5 * (B / torch.sqrt(B.square().mean(1, keepdim=True) + 1e-6)) * post.double() * torch.sigmoid(G) * torch.sigmoid(-G)
+    want, size = (each, each.abs()) if gate == "full" else (each.sum(0), each.abs().sum(0))
+    close(got, want, size * (1e-5 + 200 * U32) + want.abs() * half_step(t) + TINY[t], f"{m}x{c}")
+
+
 def test_adamw_norm_of_many_equal_gradients():
     """2^28 equal values, whose squares a running 32-bit sum takes in with the same rounding again and again."""
     n = 1 << 28
