@@ -99,6 +99,16 @@ Tensor workspace(uint64_t bytes, const Tensor& x) { return at::empty({(int64_t)b
 // graph that saved the tensor fails as it does behind torch's own in-place operators.
 void written(const Tensor& t) { if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version(); }
 
+// Which of an operator's tensors (bit i: the i-th, if it is there) this backward pass wants the gradient of. torch counts those
+// that are there.
+int64_t wanted(const AutogradContext* ctx, int64_t there) {
+    int64_t wants = 0;
+    size_t edge = 0;
+    for (int64_t bit = 1; bit <= there; bit <<= 1)
+        if (there & bit) wants |= ctx->needs_input_grad(edge++) ? bit : 0;
+    return wants;
+}
+
 // The gradients as a second differentiation has to see them: there is none.
 variable_list once(variable_list grads, const char* what) {
     if (!at::GradMode::is_enabled()) return grads;
@@ -147,13 +157,13 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
         linear_forward(x, w, b, res, (int)activation, y, slope);
         ctx->save_for_backward({x, w, slope});
         ctx->saved_data["activation"] = activation;
-        ctx->saved_data["wants"] = (int64_t)((x.requires_grad() ? 1 : 0) | (w.requires_grad() ? 2 : 0) | (b.defined() && b.requires_grad() ? 4 : 0) | (res.defined() && res.requires_grad() ? 8 : 0));
+        ctx->saved_data["there"] = (int64_t)(3 | (b.defined() ? 4 : 0) | (res.defined() ? 8 : 0));
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list dys) {
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &w = saved[1], &slope = saved[2];
-        const int64_t wants = ctx->saved_data["wants"].toInt();
+        const int64_t wants = wanted(ctx, ctx->saved_data["there"].toInt());
         const Tensor dy = rows_of(dys[0]);
         Tensor dx, dw, db, work;
         if (wants & 7) {
@@ -258,9 +268,9 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
         norm_forward(x, block, gate, post, pre, scale, eps, r, h);
         ctx->set_materialize_grads(false);
         ctx->save_for_backward({x, block, gate, post, pre});
-        int64_t wants = 0, bit = 1;
-        for (const Tensor* t : {&x, &block, &gate, &post, &pre}) { wants |= t->defined() && t->requires_grad() ? bit : 0; bit <<= 1; }
-        ctx->saved_data["wants"] = wants;
+        int64_t there = 0, bit = 1;
+        for (const Tensor* t : {&x, &block, &gate, &post, &pre}) { there |= t->defined() ? bit : 0; bit <<= 1; }
+        ctx->saved_data["there"] = there;
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["eps"] = eps;
         return {r, h};
@@ -270,7 +280,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
         if (!ds[0].defined() && !ds[1].defined()) return grads;
         const variable_list in = ctx->get_saved_variables();
         const Tensor &x = in[0];
-        const int64_t wants = ctx->saved_data["wants"].toInt();
+        const int64_t wants = wanted(ctx, ctx->saved_data["there"].toInt());
         const Tensor dr = ds[0].defined() ? ds[0].contiguous() : Tensor(), dh = ds[1].defined() ? ds[1].contiguous() : Tensor();
         DroneNorm c = norm_call(x, in[1], in[2], in[3], in[4], ctx->saved_data["scale"].toDouble(), ctx->saved_data["eps"].toDouble());
         c.dr = ptr(dr);

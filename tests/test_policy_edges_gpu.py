@@ -231,6 +231,41 @@ def test_linear_weight_gradient_of_a_very_wide_layer(t):
         close(dw[at:at + 4096], d.t() @ x.double(), d.abs().t() @ x.double().abs() * (half_step(t) + 4 * U32) + TINY[t], f"dw {at}")
 
 
+def test_linear_computes_only_what_a_backward_pass_asks_for():
+    """autograd.grad for some of the leaves: the others' gradients are neither allocated nor computed."""
+    m, k, n = 20000, 512, 64
+    x, w, b, _, dy = linear_case(m, k, n, torch.float32, "tanh", res=False)
+    full = torch.autograd.grad(policy.linear(x, w, b, "tanh"), [x, w, b], dy)
+    for asked in ((1,), (2,), (1, 2), (0, 1)):
+        y = policy.linear(x, w, b, "tanh")
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        had = torch.cuda.memory_allocated()
+        got = torch.autograd.grad(y, [(x, w, b)[i] for i in asked], dy)
+        peak = torch.cuda.max_memory_allocated() - had
+        assert all(torch.equal(g, full[i]) for g, i in zip(got, asked)), asked
+        if 0 not in asked:
+            c = policy.linear(x.detach(), w, b, "tanh")  # x needs no gradient at all: the same work
+            torch.cuda.reset_peak_memory_stats()
+            had = torch.cuda.memory_allocated()
+            torch.autograd.grad(c, [(x, w, b)[i] for i in asked], dy)
+            assert peak <= torch.cuda.max_memory_allocated() - had + (2 << 20), asked  # (blocks of the allocator; dx is 41 MB)
+
+
+def test_norm_computes_only_what_a_backward_pass_asks_for():
+    (x, block, gate, post, pre), dr, dh = norm_case(20000, 512, torch.float32, "full")
+    run = lambda *a: policy.norm_residual(a[0], a[1], gate=a[2], scale=0.5, post_weight=post, pre_weight=pre)  # noqa: E731
+    full = torch.autograd.grad(run(x, block, gate), [x, block, gate, post, pre], [dr, dh])
+    r, h = run(x, block, gate)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    had = torch.cuda.memory_allocated()
+    got = torch.autograd.grad([r, h], [post, pre], [dr, dh])
+    peak = torch.cuda.max_memory_allocated() - had
+    assert torch.equal(got[0], full[3]) and torch.equal(got[1], full[4])
+    assert peak < x.numel() * 4  # not one of the three large ones
+
+
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("gate", ["channel", "full"])
 @pytest.mark.parametrize("m, c", [(33, 32), (50, 200), (9, 1500)])
