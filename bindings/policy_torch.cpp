@@ -174,7 +174,8 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
             if (wants & 1) { dx = at::empty({x.size(0), x.size(1)}, x.options()); c.dx = ptr(dx); c.dx_ld = x.size(1); }
             if (wants & 2) { dw = at::empty({w.size(0), w.size(1)}, x.options()); c.dweight = ptr(dw); }
             if (wants & 4) { db = at::empty({w.size(0)}, x.options()); c.dbias = ptr(db); }
-            if (wants & 6) { work = workspace(lib.linear_workspace(&c), x); c.workspace = ptr(work); c.workspace_bytes = work.numel(); }
+            // (dx alone needs none, but streams through one where the layer is wide)
+            if ((wants & 6) || w.numel() > 128 * 128) { work = workspace(lib.linear_workspace(&c), x); c.workspace = ptr(work); c.workspace_bytes = work.numel(); }
             run(lib.linear_backward(&c, stream_of(x)));
         }
         return once({dx, dw, db, wants & 8 ? dys[0] : Tensor(), Tensor()}, "linear");

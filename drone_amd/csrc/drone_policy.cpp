@@ -162,9 +162,9 @@ int drone_linear_backward(const DroneLinear* c, void* stream) {
     if (odd(c->x, m) || odd(c->weight, m) || odd(c->dy, m) || odd(c->slope, m) || odd(c->dx, m) || odd(c->dweight, m) || odd(c->dbias, m)) return fail(what, "a pointer is not aligned to its elements"), -1;
     LinearArgs a = linear_args(c);
     if (c->activation == DRONE_ACTIVATION_NONE) a.slope = nullptr;
-    if (c->dweight || c->dbias) {
-        if (!c->workspace || odd(c->workspace, 15) || c->workspace_bytes < linear_work_bytes(c->dtype, c->rows, a.in, a.out))
-            return fail(what, "dweight and dbias need drone_linear_workspace bytes, 16-byte aligned"), -1;
+    if (!c->workspace || odd(c->workspace, 15) || c->workspace_bytes < linear_work_bytes(c->dtype, c->rows, a.in, a.out)) {
+        if (c->dweight || c->dbias) return fail(what, "dweight and dbias need drone_linear_workspace bytes, 16-byte aligned"), -1;
+        a.work = nullptr;
     }
     OnDevice dev(c->device);
     return dev.ok ? launched(linear_backward_launch(c->dtype, a, (hipStream_t)stream), what) : -1;

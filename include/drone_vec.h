@@ -384,7 +384,9 @@ int drone_vec_copy_to_host(DroneVec* v, void* host_dst, const void* device_src, 
  * that are not NULL (dweight [out][in] and dbias [out] dense); the residual's gradient is dy itself. y may be the residual
  * (same pointer and leading dimension); no other output may overlap an input. rows 0 ... 2^30 (0: sums are zero),
  * in / out 1 ... 65536. Backward with dweight or dbias needs drone_linear_workspace bytes at `workspace` (16-byte aligned):
- * partial sums, and for wide or odd layers dz and copies laid out in whole pieces (up to about rows (in + out) elements). */
+ * partial sums, and for wide or odd layers dz and copies laid out in whole pieces (up to about rows (in + out) elements; the
+ * size goes by rows, in, out and dtype alone, so that it has room for any alignment). dx alone takes none, and of a wide layer
+ * is faster with it. */
 typedef struct DroneLinear {
     uint32_t struct_size; /* = sizeof(DroneLinear) */
     int32_t device, dtype, activation;

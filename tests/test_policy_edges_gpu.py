@@ -313,3 +313,15 @@ def test_linear_gradient_of_saturated_units(t, act, m, n):
     want = 2.0 ** 12 * s
     tol = want.abs() * (2 * half_step(t) + (2.0 ** -11 if t == torch.bfloat16 else 0) + 1e-5)
     close(dx, want, tol, f"{act} {m}x{n}")
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m, k, n", [(66001, 264, 520), (20001, 520, 384), (9001, 1024, 520)])
+@pytest.mark.parametrize("act", ["none", "silu"])
+def test_linear_input_gradient_alone_of_a_wide_layer(t, m, k, n, act):
+    """Asked for alone it takes the same form as beside the weights', so it has the same bits."""
+    x, w, b, _, dy = linear_case(m, k, n, t, act, res=False)
+    y = policy.linear(x, w, b, act)
+    full = torch.autograd.grad(y, [x, w, b], dy, retain_graph=True)
+    alone, = torch.autograd.grad(y, [x], dy)
+    assert torch.equal(alone, full[0])
