@@ -339,6 +339,7 @@ Tensor adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& 
                   std::pair<double, double> betas, double eps, double weight_decay, std::optional<double> max_grad_norm, const std::optional<std::vector<Tensor>>& masters) {
     TORCH_CHECK_VALUE(!params.empty(), "no parameters");
     not_traced("adamw_step");
+    TORCH_CHECK_VALUE(!max_grad_norm || *max_grad_norm > 0, "max_grad_norm must be positive (None: no clipping), got ", *max_grad_norm);
     const Tensor& first = params[0];
     const int dtype = dtype_of(first, "params[0]");
     TORCH_CHECK_VALUE(masters.has_value() == (dtype != DRONE_F32), "16-bit params need float32 masters, float32 params have none");

@@ -217,6 +217,7 @@ int drone_adamw_step(const DroneAdamW* c, void* stream) {
     // the update multiplies m by rcp(sqrt(v) + eps) of the hardware, which take denormals for 0: without eps that is infinite
     if (!((float)c->eps >= FLT_MIN)) return fail(what, "eps must be positive (a normal 32-bit number)"), -1;
     if (c->max_grad_norm != c->max_grad_norm) return fail(what, "max_grad_norm is not a number"), -1;
+    if (c->max_grad_norm > 0 && (float)c->max_grad_norm < FLT_MIN) return fail(what, "max_grad_norm must be a normal 32-bit number (or not positive: no clipping)"), -1;
     const uintptr_t m = elem_mask(c->dtype);
     for (int i = 0; i < c->count; i++) {
         const DroneAdamWTensor& t = c->tensors[i];

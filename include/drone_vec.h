@@ -424,7 +424,7 @@ int drone_norm_backward(const DroneNorm* call, void* hip_stream);
 uint64_t drone_norm_workspace(const DroneNorm* call);
 
 /* One AdamW step over `count` tensors, clipped by the global norm of their gradients:
- *   c = min(1, max_grad_norm / (sqrt(sum g^2) + 1e-6)) (1 if max_grad_norm <= 0);  g' = c g
+ *   c = min(1, max_grad_norm / (sqrt(sum g^2) + 1e-6)) (1 if max_grad_norm <= 0; else a normal f32);  g' = c g
  *   m = beta1 m + (1 - beta1) g';  v = beta2 v + (1 - beta2) g'^2
  *   p = p (1 - lr weight_decay) - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps)
  * p and g of `dtype`, m and v f32, master f32 (required for the 16-bit types, whose p is the rounded master: a p that is
