@@ -344,7 +344,7 @@ Tensor adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& 
     const int dtype = dtype_of(first, "params[0]");
     TORCH_CHECK_VALUE(masters.has_value() == (dtype != DRONE_F32), "16-bit params need float32 masters, float32 params have none");
     const size_t count = params.size();
-    std::vector<const void*> seen;
+    std::vector<std::pair<const char*, const char*>> seen;  // first byte, one past the last
     seen.reserve(5 * count);
     auto check_list = [&](const char* name, const std::vector<Tensor>& list, at::ScalarType type) {
         TORCH_CHECK_VALUE(list.size() == count, list.size(), " ", name, " for ", count, " params");
@@ -352,7 +352,7 @@ Tensor adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& 
             const Tensor& t = list[i];
             TORCH_CHECK_VALUE(t.scalar_type() == type && t.device() == first.device() && t.sizes() == params[i].sizes() && t.is_contiguous(), name, ": expected a contiguous ", type,
                               " tensor of shape ", params[i].sizes(), " on ", first.device(), ", got ", t.scalar_type(), " ", t.sizes(), " on ", t.device());
-            if (t.numel()) seen.push_back(t.data_ptr());
+            if (t.numel()) seen.emplace_back((const char*)t.data_ptr(), (const char*)t.data_ptr() + t.numel() * t.element_size());
         }
     };
     check_list("params", params, first.scalar_type());
@@ -361,7 +361,10 @@ Tensor adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& 
     check_list("exp_avg_sqs", exp_avg_sqs, at::kFloat);
     if (masters) check_list("masters", *masters, at::kFloat);
     std::sort(seen.begin(), seen.end());
-    TORCH_CHECK_VALUE(std::adjacent_find(seen.begin(), seen.end()) == seen.end(), "a tensor is there twice");
+    for (size_t i = 1; i < seen.size(); i++) {
+        TORCH_CHECK_VALUE(seen[i].first != seen[i - 1].first, "a tensor is there twice");
+        TORCH_CHECK_VALUE(seen[i].first >= seen[i - 1].second, "two tensors overlap");
+    }
     TORCH_CHECK_VALUE(step.scalar_type() == at::kInt && step.numel() == 1 && step.device() == first.device(), "step must be an int32 tensor of one element on the params' device");
     std::vector<DroneAdamWTensor> table(count);
     for (size_t i = 0; i < count; i++)

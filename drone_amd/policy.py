@@ -69,7 +69,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.
 
     params and grads of one type; exp_avgs, exp_avg_sqs float32; 16-bit params need float32 ``masters`` (the params are
     their rounded copies; a value that is not has been written since, and the step starts from it). ``step``: int32 tensor ``[1]`` on the device, the steps done so far; the call adds 1, so a step
-    captured into a graph replays with an advancing count. All tensors contiguous, on one GPU, none twice."""
+    captured into a graph replays with an advancing count. All tensors contiguous, on one GPU, none twice or over another."""
     return _native().adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas, eps, weight_decay, max_grad_norm, masters)
 
 

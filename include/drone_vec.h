@@ -431,7 +431,7 @@ uint64_t drone_norm_workspace(const DroneNorm* call);
  * not has been written since the last step, and the step starts from it; NULL for DRONE_F32), each dense with `elements` values. `step` (device, one int32) counts the steps done: the call adds 1 and t is
  * the result, so a captured call replays with an advancing t (lr and the rest stay those of the capture). `grad_norm`
  * (device, one f32) or NULL receives the norm before clipping. `tensors` is host memory, read during the call. No tensor
- * may appear twice; elements 0 ... 2^34; eps > 0 and a normal f32. drone_adamw_workspace bytes at `workspace`. */
+ * may appear twice or overlap another; elements 0 ... 2^34; eps > 0 and a normal f32. drone_adamw_workspace bytes at `workspace`. */
 typedef struct DroneAdamWTensor {
     void* param;
     const void* grad;

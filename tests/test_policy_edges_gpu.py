@@ -266,6 +266,19 @@ def test_norm_computes_only_what_a_backward_pass_asks_for():
     assert peak < x.numel() * 4  # not one of the three large ones
 
 
+def test_adamw_refuses_tensors_that_overlap():
+    flat = torch.zeros(300, device="cuda")
+    s = adamw_case([(100,), (100,)], torch.float32)
+    call = lambda **o: policy.adamw_step(**{**dict(params=s["params"], grads=s["grads"], exp_avgs=s["m"], exp_avg_sqs=s["v"], step=s["step"], lr=1e-3), **o})  # noqa: E731
+    with pytest.raises(ValueError, match="overlap"):
+        call(params=[flat[:100], flat[99:199]])
+    with pytest.raises(ValueError, match="overlap"):
+        call(exp_avgs=[flat[:100], flat[100:200]], exp_avg_sqs=[flat[199:299], s["v"][1]])
+    assert not flat.any()
+    call(params=[flat[:100], flat[100:200]])  # neighbours are not the same
+    assert flat[:200].all() and not flat[200:].any()
+
+
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("gate", ["channel", "full"])
 @pytest.mark.parametrize("m, c", [(33, 32), (50, 200), (9, 1500)])
