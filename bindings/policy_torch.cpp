@@ -78,12 +78,15 @@ void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 bool good_rows(const Tensor& t) { return t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1)); }
 
 // A tensor [..., n] as [rows][n] with contiguous rows and a leading dimension of at least n: a view where there is one,
-// else a copy. Overlapping rows (an expanded tensor) are copied.
+// else a copy. Overlapping rows (an expanded tensor) are copied, and so is a view whose sign is still to be taken.
 Tensor rows_of(const Tensor& t) {
+    if (t.defined() && t.is_neg()) return rows_of(t.resolve_neg());
     if (!t.defined() || good_rows(t)) return t;
     const Tensor r = t.dim() == 2 ? t : t.reshape({t.numel() / std::max<int64_t>(1, t.size(-1)), t.size(-1)});
     return good_rows(r) ? r : r.contiguous();
 }
+
+Tensor dense(const Tensor& t) { return t.resolve_neg().contiguous(); }
 
 int64_t ld(const Tensor& t) { return !t.defined() ? 0 : t.size(0) > 1 ? std::max(t.stride(0), t.size(1)) : t.size(1); }
 
@@ -208,12 +211,12 @@ Tensor linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, cons
     if (has(bias)) check("bias", *bias, {n}, x);
     if (has(residual)) check("residual", *residual, shape, x);
     const bool learn = at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || (has(bias) && bias->requires_grad()) || (has(residual) && residual->requires_grad()));
-    const Tensor x2 = rows_of(x), w2 = rows_of(weight), b2 = has(bias) ? bias->contiguous() : Tensor(), r2 = has(residual) ? rows_of(*residual) : Tensor();
+    const Tensor x2 = rows_of(x), w2 = rows_of(weight), b2 = has(bias) ? dense(*bias) : Tensor(), r2 = has(residual) ? rows_of(*residual) : Tensor();
     if (has(out)) {
         check("out", *out, shape, x);
         TORCH_CHECK_VALUE(!learn && !(at::GradMode::is_enabled() && out->requires_grad()), "out= cannot be differentiated: call under torch.no_grad()");
         const Tensor o = flat ? *out : out->view({x2.size(0), n});
-        TORCH_CHECK_VALUE(good_rows(o), "out must have contiguous rows that do not overlap");
+        TORCH_CHECK_VALUE(good_rows(o) && !o.is_neg(), "out must have contiguous rows that do not overlap");
         const bool in_place = r2.defined() && r2.data_ptr() == o.data_ptr() && ld(r2) == ld(o);
         TORCH_CHECK_VALUE(!overlap(x2, o) && !overlap(w2, o) && !(b2.defined() && overlap(b2.unsqueeze(0), o)) && (in_place || !overlap(r2, o)),
                           "out overlaps an input (only the residual may be updated in place)");
@@ -282,7 +285,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
         const variable_list in = ctx->get_saved_variables();
         const Tensor &x = in[0];
         const int64_t wants = wanted(ctx, ctx->saved_data["there"].toInt());
-        const Tensor dr = ds[0].defined() ? ds[0].contiguous() : Tensor(), dh = ds[1].defined() ? ds[1].contiguous() : Tensor();
+        const Tensor dr = ds[0].defined() ? dense(ds[0]) : Tensor(), dh = ds[1].defined() ? dense(ds[1]) : Tensor();
         DroneNorm c = norm_call(x, in[1], in[2], in[3], in[4], ctx->saved_data["scale"].toDouble(), ctx->saved_data["eps"].toDouble());
         c.dr = ptr(dr);
         c.dh = ptr(dh);
@@ -317,18 +320,18 @@ std::tuple<Tensor, Tensor> norm_residual(const Tensor& x, const OptTensor& block
     TORCH_CHECK_VALUE(eps >= 0, "eps must not be negative");
     auto learns = [](const OptTensor& t) { return has(t) && t->requires_grad(); };
     const bool learn = at::GradMode::is_enabled() && (x.requires_grad() || learns(block) || learns(gate) || learns(post_weight) || learns(pre_weight)), flat = x.dim() == 2;
-    auto dense = [](const OptTensor& t) { return has(t) ? t->contiguous() : Tensor(); };
+    auto weight = [](const OptTensor& t) { return has(t) ? dense(*t) : Tensor(); };
     const auto two = [](const Tensor& t) { return t.dim() == 1 ? t.unsqueeze(0) : t; };
-    const Tensor x2 = rows_of(two(x)), block2 = has(block) ? rows_of(two(*block)) : Tensor(), gate2 = channel ? gate->contiguous() : has(gate) ? rows_of(two(*gate)) : Tensor();
+    const Tensor x2 = rows_of(two(x)), block2 = has(block) ? rows_of(two(*block)) : Tensor(), gate2 = channel ? dense(*gate) : has(gate) ? rows_of(two(*gate)) : Tensor();
     Tensor r, h;
     if (learn) {
-        const variable_list out = NormFunction::apply(x2, opt(block2), opt(gate2), opt(dense(post_weight)), opt(dense(pre_weight)), scale, eps);
+        const variable_list out = NormFunction::apply(x2, opt(block2), opt(gate2), opt(weight(post_weight)), opt(weight(pre_weight)), scale, eps);
         r = out[0];
         h = out[1];
     } else {
         r = at::empty({x2.size(0), width}, x.options());
         h = at::empty({x2.size(0), width}, x.options());
-        norm_forward(x2, block2, gate2, dense(post_weight), dense(pre_weight), scale, eps, r, h);
+        norm_forward(x2, block2, gate2, weight(post_weight), weight(pre_weight), scale, eps, r, h);
     }
     return flat ? std::make_tuple(r, h) : std::make_tuple(r.view(x.sizes()), h.view(x.sizes()));
 }
@@ -350,7 +353,7 @@ Tensor adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& 
         TORCH_CHECK_VALUE(list.size() == count, list.size(), " ", name, " for ", count, " params");
         for (size_t i = 0; i < count; i++) {
             const Tensor& t = list[i];
-            TORCH_CHECK_VALUE(t.scalar_type() == type && t.device() == first.device() && t.sizes() == params[i].sizes() && t.is_contiguous(), name, ": expected a contiguous ", type,
+            TORCH_CHECK_VALUE(t.scalar_type() == type && t.device() == first.device() && t.sizes() == params[i].sizes() && t.is_contiguous() && !t.is_neg(), name, ": expected a contiguous ", type,
                               " tensor of shape ", params[i].sizes(), " on ", first.device(), ", got ", t.scalar_type(), " ", t.sizes(), " on ", t.device());
             if (t.numel()) seen.emplace_back((const char*)t.data_ptr(), (const char*)t.data_ptr() + t.numel() * t.element_size());
         }

@@ -279,6 +279,33 @@ def test_adamw_refuses_tensors_that_overlap():
     assert flat[:200].all() and not flat[200:].any()
 
 
+def test_negated_views_count_as_what_they_are():
+    """A conjugate's imaginary part is a view whose sign waits to be taken: by address it is the other sign."""
+    x, w, b, r, dy = linear_case(9, 16, 8, torch.float32, "tanh")
+    flip = lambda v: torch._neg_view(v.detach().neg())  # noqa: E731
+    assert flip(x).is_neg() and torch.equal(flip(x), x)
+    want = policy.linear(x, w, b, "tanh", r)
+    for at in range(4):
+        a = [v.detach() for v in (x, w, b, r)]
+        a[at] = flip(a[at])
+        assert torch.equal(policy.linear(a[0], a[1], a[2], "tanh", a[3]), want), at
+    leaf = x.detach().neg().requires_grad_(True)
+    dx, = torch.autograd.grad(policy.linear(torch._neg_view(leaf), w, b, "tanh", r), leaf, flip(dy))
+    assert torch.equal(dx, torch.autograd.grad(want, x, dy)[0].neg())
+    ts, dr, dh = norm_case(9, 16, torch.float32, "full", leaf=False)
+    keep = policy.norm_residual(ts[0], ts[1], gate=ts[2], post_weight=ts[3], pre_weight=ts[4])
+    for at in range(5):
+        a = list(ts)
+        a[at] = flip(a[at])
+        got = policy.norm_residual(a[0], a[1], gate=a[2], post_weight=a[3], pre_weight=a[4])
+        assert torch.equal(got[0], keep[0]) and torch.equal(got[1], keep[1]), at
+    s = adamw_case([(7,)], torch.float32)
+    with pytest.raises(ValueError, match="contiguous"):
+        policy.adamw_step(s["params"], [flip(s["grads"][0])], s["m"], s["v"], s["step"], lr=1e-3)
+    with torch.no_grad(), pytest.raises(ValueError, match="out"):
+        policy.linear(x, w, b, out=torch._neg_view(torch.zeros(9, 8, device="cuda")))
+
+
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("gate", ["channel", "full"])
 @pytest.mark.parametrize("m, c", [(33, 32), (50, 200), (9, 1500)])
