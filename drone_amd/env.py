@@ -143,6 +143,8 @@ class Drone:
             bufs = self._collected = vec.alloc_step_many(K)
         own = vec.actions, (vec.observations, vec.rewards, vec.terminals, vec.truncations)
         vec.use_torch_stream()
+        done = 0
+        before = self.tick
         try:
             with torch.no_grad():
                 bufs.observations[0].copy_(own[1][0])
@@ -151,16 +153,20 @@ class Drone:
                     vec.bind_actions(bufs.actions[k])
                     vec.bind_outputs(bufs.observations[k + 1] if k + 1 < K else own[1][0], bufs.rewards[k], bufs.terminals[k], bufs.truncations[k])
                     vec.step()
-                own[0].copy_(bufs.actions[K - 1])
-                for mine, block in zip(own[1][1:], (bufs.rewards, bufs.terminals, bufs.truncations)):
-                    mine.copy_(block[K - 1])
-            # the kernels wrote by address: a graph that saved one of these tensors must not be differentiated after this
-            torch.autograd.graph.increment_version((bufs.observations, bufs.actions, bufs.rewards, bufs.terminals, bufs.truncations, *own[1]))
-        finally:
+                    done = k + 1
+        finally:  # (a policy that raises leaves the env where the steps before it did)
             vec.bind_actions(own[0])
             vec.bind_outputs(*own[1])
-        before = self.tick
-        self.tick += K
+            self.tick += done
+            with torch.no_grad():
+                if 0 < done < K:
+                    own[1][0].copy_(bufs.observations[done])
+                if done:
+                    own[0].copy_(bufs.actions[done - 1])
+                    for mine, block in zip(own[1][1:], (bufs.rewards, bufs.terminals, bufs.truncations)):
+                        mine.copy_(block[done - 1])
+            # the kernels wrote by address: a graph that saved one of these tensors must not be differentiated after this
+            torch.autograd.graph.increment_version((bufs.observations, bufs.actions, bufs.rewards, bufs.terminals, bufs.truncations, *own[1]))
         infos = []
         if self.log_interval and before // self.log_interval != self.tick // self.log_interval:
             log = vec.log()

@@ -306,6 +306,42 @@ def test_negated_views_count_as_what_they_are():
         policy.linear(x, w, b, out=torch._neg_view(torch.zeros(9, 8, device="cuda")))
 
 
+def test_collect_stopped_by_its_policy(hip):
+    """A policy that raises in the middle: the env and its buffers are where as many step calls leave them."""
+    from drone_amd.env import Drone
+
+    net = policy.Policy(width=32, device="cuda:0")
+    a, b = (Drone(num_envs=501, task="waypoint", device="cuda:0", seed=4, log_interval=0, horizon=9) for _ in range(2))
+    for e in (a, b):
+        e.reset(4)
+    calls = []
+
+    def stops(obs, out):
+        calls.append(1)
+        if len(calls) == 5:
+            raise KeyboardInterrupt
+        return net(obs, out=out)
+
+    a.collect(net, 6)
+    with pytest.raises(KeyboardInterrupt):
+        a.collect(stops, 6)
+    for _ in range(6 + 4):
+        with torch.no_grad():
+            net(b.observations, out=b.actions)
+        b.step(b.actions)
+    for name in ("observations", "actions", "rewards", "terminals", "truncations"):
+        assert torch.equal(getattr(a, name), getattr(b, name)), name
+    assert a.tick == b.tick and a.vec.gstep == b.vec.gstep
+    a.collect(net, 2)
+    for _ in range(2):
+        with torch.no_grad():
+            net(b.observations, out=b.actions)
+        b.step(b.actions)
+    assert torch.equal(a.observations, b.observations) and torch.equal(a.rewards, b.rewards)
+    for e in (a, b):
+        e.close()
+
+
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("gate", ["channel", "full"])
 @pytest.mark.parametrize("m, c", [(33, 32), (50, 200), (9, 1500)])
