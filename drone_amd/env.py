@@ -130,7 +130,8 @@ class Drone:
         the env's current observations and its actions go straight into the block the env steps from. Returns K-major
         ``(observations [K][N][O] the policy saw, actions [K][N][4], rewards, terminals, truncations [K][N], infos)``; the
         blocks are reused from call to call for the same K. Afterwards the env and its per-step buffers are where K calls of
-        ``step`` leave them. Device buffers only; capturable after ``vec.enable_graph_capture`` (one call outside first)."""
+        ``step`` leave them. Device buffers only; capturable after ``vec.enable_graph_capture``, with one call outside first on the
+        captured stream: ``tick`` and the log stand still in the captured call and its replays."""
         import torch
 
         vec, K = self.vec, int(k_steps)
@@ -157,7 +158,10 @@ class Drone:
         finally:  # (a policy that raises leaves the env where the steps before it did)
             vec.bind_actions(own[0])
             vec.bind_outputs(*own[1])
-            self.tick += done
+            if torch.cuda.is_current_stream_capturing():
+                self._captured = [*getattr(self, "_captured", []), bufs]  # the replays write these blocks, whatever K comes next
+            else:
+                self.tick += done
             with torch.no_grad():
                 if 0 < done < K:
                     own[1][0].copy_(bufs.observations[done])

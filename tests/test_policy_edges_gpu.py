@@ -401,3 +401,47 @@ def test_linear_input_gradient_alone_of_a_wide_layer(t, m, k, n, act):
     full = torch.autograd.grad(y, [x, w, b], dy, retain_graph=True)
     alone, = torch.autograd.grad(y, [x], dy)
     assert torch.equal(alone, full[0])
+
+
+def test_captured_collect_replays(hip):
+    """collect in one graph, replayed with the program's own work in between, against the same calls made eagerly. The log's
+    interval passes inside the captured call: it cannot be read there, and is read by the next eager one."""
+    from drone_amd.env import Drone
+
+    net = policy.Policy(width=32, device="cuda:0")
+    a, b = (Drone(num_envs=777, task="waypoint", device="cuda:0", seed=6, log_interval=4, horizon=9) for _ in range(2))
+    for e in (a, b):
+        e.reset(6)
+    a.vec.enable_graph_capture(True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        a.collect(net, 4)
+    torch.cuda.synchronize()
+    b.collect(net, 4)
+    g = torch.cuda.CUDAGraph()
+    tick = a.tick
+    with torch.cuda.graph(g, stream=side):
+        blocks = a.collect(net, 4)
+    assert blocks[5] == [] and a.tick == tick  # nothing has run yet
+    for k in range(5):
+        g.replay()
+        torch.cuda.synchronize()
+        want = b.collect(net, 4)
+        torch.cuda.synchronize()
+        for x, y in zip(blocks[:5], want[:5]):
+            assert torch.equal(x, y), k
+        assert torch.equal(a.observations, b.observations) and torch.equal(a.actions, b.actions) and torch.equal(a.truncations, b.truncations), k
+        assert a.vec.gstep == b.vec.gstep
+    infos = a.collect(net, 4)[5]
+    assert len(infos) == 1 and infos[0]["n"] > 0
+    # another K: the captured blocks stay the graph's own, whoever else has let go of them
+    shape = blocks[0].shape
+    del blocks, x, y
+    a.collect(net, 2)
+    others = [torch.full(shape, 7.0, device="cuda") for _ in range(8)]
+    g.replay()
+    torch.cuda.synchronize()
+    assert all((o == 7).all() for o in others)
+    for e in (a, b):
+        e.close()
