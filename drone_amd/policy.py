@@ -86,8 +86,8 @@ class AdamW(torch.optim.Optimizer):
     """``adamw_step`` as a torch optimizer: one parameter group's tensors of one type per step call, moments and (for 16-bit
     parameters) masters in float32. Weights may be written between steps (a loaded state, a target network's copy): the next
     step starts from what is there. ``max_grad_norm`` clips by the norm over a whole group; ``grad_norm`` holds the last
-    step's norms, one ``[1]`` tensor per group. Parameters without a gradient are left alone; the step count is the
-    group's. ``lr`` and the rest are read at every call (a captured step keeps those of its capture)."""
+    step's norms, one ``[1]`` tensor per group (None where no parameter had a gradient). Parameters without a gradient are
+    left alone; the step count is the group's. ``lr`` and the rest are read at every call (a captured step keeps those of its capture)."""
 
     def __init__(self, params, lr=3e-4, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, max_grad_norm=None):
         if lr < 0 or weight_decay < 0 or not eps > 0 or not all(0 <= b < 1 for b in betas):
@@ -140,6 +140,7 @@ class AdamW(torch.optim.Optimizer):
         for group in self.param_groups:
             params = [p for p in group["params"] if p.grad is not None]
             if not params:
+                self.grad_norm.append(None)
                 continue
             states = [self.state[p] for p in params]
             masters = [s["master"] for s in states] if params[0].dtype != torch.float32 else None

@@ -369,6 +369,16 @@ def test_adamw_norm_of_many_equal_gradients():
     assert abs(norm.item() - want) <= 64 * U32 * want
 
 
+def test_optimizer_reports_a_norm_for_every_group():
+    ps = [torch.nn.Parameter(rand(9, seed=i)) for i in range(3)]
+    opt = policy.AdamW([{"params": [p]} for p in ps])
+    ps[0].grad, ps[2].grad = torch.ones(9, device="cuda"), torch.full((9,), 2.0, device="cuda")
+    opt.step()
+    assert opt.grad_norm[1] is None  # no gradient in the group: no step, no norm
+    assert [opt.grad_norm[i].item() for i in (0, 2)] == [3.0, 6.0]
+    assert [g["step"].item() for g in opt.param_groups] == [1, 0, 1]
+
+
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("act", ["tanh", "silu"])
 @pytest.mark.parametrize("m, n", FORMS)
