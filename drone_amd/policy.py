@@ -30,7 +30,7 @@ def _native():
             from . import policy_torch
         except ImportError as e:
             raise RuntimeError("drone_amd/policy_torch is missing or does not load: build it first "
-                               f"(python -c 'import __graft_entry__ as g; g.build()' or make -C bindings): {e}") from e
+                               f"(python -c 'import __graft_entry__ as g; g.build()' or make -C bindings policy): {e}") from e
         names = [n for n in abi.SYMBOLS if n.startswith(("drone_linear", "drone_norm", "drone_adamw"))] + ["drone_last_error"]
         policy_torch.bind({n: C.cast(getattr(lib, n), C.c_void_p).value for n in names})
         _native_module = policy_torch
