@@ -6,6 +6,8 @@
 #include <torch/extension.h>
 
 #include <c10/hip/HIPStream.h>
+#include <hip/hip_runtime_api.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
@@ -112,6 +114,20 @@ int64_t wanted(const AutogradContext* ctx, int64_t there) {
     return wants;
 }
 
+// In a backward pass: a captured one may hand nothing to a leaf's accumulator that an eager graph of the default stream still
+// holds. It would run on that stream, where a capture cannot follow, and torch ends the process over it.
+void capturable(const Tensor& x, const char* what) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(c10::hip::getCurrentHIPStream(x.get_device()), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    const auto node = torch::autograd::get_current_node();
+    for (size_t i = 0; i < node->num_outputs(); i++) {
+        const auto& leaf = node->next_edge(i).function;
+        if (!dynamic_cast<const torch::autograd::AccumulateGrad*>(leaf.get()) || !node->task_should_compute_output(i)) continue;
+        const auto stream = leaf->stream();
+        TORCH_CHECK(!stream || stream->id() != 0, what, ": a graph built on the default stream still holds a leaf of this captured backward pass; let go of it (del loss) before the capture");
+    }
+}
+
 // The gradients as a second differentiation has to see them: there is none.
 variable_list once(variable_list grads, const char* what) {
     if (!at::GradMode::is_enabled()) return grads;
@@ -166,6 +182,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
     static variable_list backward(AutogradContext* ctx, variable_list dys) {
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &w = saved[1], &slope = saved[2];
+        capturable(x, "linear");
         const int64_t wants = wanted(ctx, ctx->saved_data["there"].toInt());
         const Tensor dy = rows_of(dys[0]);
         Tensor dx, dw, db, work;
@@ -284,6 +301,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
         if (!ds[0].defined() && !ds[1].defined()) return grads;
         const variable_list in = ctx->get_saved_variables();
         const Tensor &x = in[0];
+        capturable(x, "norm_residual");
         const int64_t wants = wanted(ctx, ctx->saved_data["there"].toInt());
         const Tensor dr = ds[0].defined() ? dense(ds[0]) : Tensor(), dh = ds[1].defined() ? dense(ds[1]) : Tensor();
         DroneNorm c = norm_call(x, in[1], in[2], in[3], in[4], ctx->saved_data["scale"].toDouble(), ctx->saved_data["eps"].toDouble());

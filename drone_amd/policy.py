@@ -9,8 +9,9 @@ cost. Three operators over the C-ABI of ``include/drone_vec.h``, each one or two
 * ``adamw_step``: clip by the global gradient norm and the AdamW update of all tensors (``drone_adamw_step``)
 
 and over them ``Linear``, ``Policy`` and ``AdamW`` for torch programs. Tensors are float32, bfloat16 or float16 on one GPU;
-sums, statistics and moments are held in 32 bits. There is no CPU path. The reference snapshot holds no policy or trainer
-source to cite (``/root/reference/.gitmodules:1-3``).
+sums, statistics and moments are held in 32 bits. There is no CPU path. Every call can be captured into a graph; a captured
+backward pass is refused where a graph built on the default stream still holds one of its leaves (an eager loss: let go of
+it). The reference snapshot holds no policy or trainer source to cite (``/root/reference/.gitmodules:1-3``).
 """
 import ctypes as C
 

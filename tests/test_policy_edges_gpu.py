@@ -455,3 +455,40 @@ def test_captured_collect_replays(hip):
     assert all((o == 7).all() for o in others)
     for e in (a, b):
         e.close()
+
+
+@pytest.mark.parametrize("op", ["linear", "norm"])
+def test_a_backward_pass_is_not_captured_beside_an_eager_graph_of_its_leaves(op):
+    """Leaves' gradients go to accumulators that live as long as a graph holds them. One that an eager graph on the default
+    stream holds runs there, where a captured pass cannot follow: refused before it gets there, and the capture ends whole.
+    Without that graph the same capture goes through."""
+    if op == "linear":
+        x, w, b, _, dy = linear_case(700, 24, 32, torch.float32, "tanh", res=False)
+        leaves, run, ds = [w, b], (lambda: [policy.linear(x, w, b, "tanh")]), [dy]
+    else:
+        (x, block, gate, post, pre), dr, dh = norm_case(700, 32, torch.float32, "channel")
+        leaves, run, ds = [gate, post, pre], (lambda: list(policy.norm_residual(x, block, gate=gate, post_weight=post, pre_weight=pre))), [dr, dh]
+    held = run()
+    want = torch.autograd.grad(held, leaves, ds, retain_graph=True)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="default stream"):
+        with torch.cuda.graph(g):
+            torch.autograd.grad(run(), leaves, ds)
+    if op == "linear":  # a captured pass that asks for another leaf only has nothing to hand to those
+        other = x.detach().clone().requires_grad_(True)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            dx, = torch.autograd.grad(policy.linear(other, w, b, "tanh"), other, dy)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(dx, torch.autograd.grad(policy.linear(other, w, b, "tanh"), other, dy)[0])
+    assert torch.equal(torch.autograd.grad(held, leaves, ds)[0], want[0])  # nothing else is the worse for it
+    del held
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = torch.autograd.grad(run(), leaves, ds)
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
