@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from drone_amd import policy
-from test_policy_gpu import HYPER, MLP, TINY, TYPES, U32, adamw_case, check_norm, close, half_step, linear_case, norm_case, rand, step
+from test_policy_gpu import HYPER, MLP, TINY, TYPES, U32, adamw_case, check_linear, check_norm, close, half_step, linear_case, norm_case, rand, step
 
 pytestmark = pytest.mark.gpu
 
@@ -229,6 +229,14 @@ def test_linear_weight_gradient_of_a_very_wide_layer(t):
     for at in range(0, n, 4096):
         d = dy[:, at:at + 4096].double()
         close(dw[at:at + 4096], d.t() @ x.double(), d.abs().t() @ x.double().abs() * (half_step(t) + 4 * U32) + TINY[t], f"dw {at}")
+
+
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m, k, n", [(66001, 520, 264), (66001, 1032, 520), (66001, 264, 520), (66001, 261, 523)])
+def test_linear_wide_streaming_form(t, m, k, n):
+    """Sizes at which 256 x 256 tiles stream, forward (reductions over 1 KiB a row) and input gradient (264 and 261 by 520
+    and more), with a last row tile, feature tile and reduction step that are not whole; the last pair is laid out first."""
+    check_linear(*linear_case(m, k, n, t, "silu"), "silu", f"{m}x{k}x{n}")
 
 
 def test_linear_computes_only_what_a_backward_pass_asks_for():
