@@ -9,10 +9,10 @@ keeps the step counter in HBM so the replays advance it. Last: the same graph
 with a frame skip of 4 — one policy forward, then four env steps under that
 action in ONE launch (drone_vec_step_repeat), the policy reading the last of the
 four observation blocks. Then the same loop with the library's own layers
-(drone_amd.policy: one launch a layer), and a learner on top of it: Drone.collect,
-the gradient, one AdamW step.
+(drone_amd.policy: one launch a layer; --blocks: norms around gated residual
+blocks), and a learner on top of it: Drone.collect, the gradient, one AdamW step.
 
-    python examples/torch_policy_loop.py [--envs 65536] [--steps 500] [--task hover]
+    python examples/torch_policy_loop.py [--envs 65536] [--steps 500] [--task hover] [--blocks 0]
 """
 import argparse
 import os
@@ -32,6 +32,7 @@ def main():
     ap.add_argument("--steps", type=int, default=500)
     ap.add_argument("--task", default="hover")
     ap.add_argument("--hidden", type=int, default=64)
+    ap.add_argument("--blocks", type=int, default=0, help="gated residual blocks of the drone_amd.policy network (0: plain hidden layers)")
     ap.add_argument("--skip", type=int, default=4, help="frame skip of the last loop (env steps per policy step)")
     a = ap.parse_args()
     dev = torch.device("cuda:0")
@@ -117,7 +118,7 @@ def main():
     # the same network on the library's own layers (drone_amd.policy), captured the same way: four launches a step
     from drone_amd.policy import AdamW, Policy
 
-    policy = Policy(vec.observations.shape[1], a.hidden, device=dev)
+    policy = Policy(vec.observations.shape[1], a.hidden, blocks=a.blocks, device=dev)
     with torch.no_grad():
         with torch.cuda.stream(side):
             vec.use_torch_stream()

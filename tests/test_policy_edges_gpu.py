@@ -1,6 +1,9 @@
 """The policy operators at the edges of what they allow: calls that the other tests do not make, each against 64-bit
 formulas, against the same work done another way, or refused."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -8,6 +11,7 @@ import torch
 from drone_amd import policy
 from test_policy_gpu import HYPER, MLP, TINY, TYPES, U32, adamw_case, check_linear, check_norm, close, half_step, linear_case, norm_case, rand, step
 
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 pytestmark = pytest.mark.gpu
 
 
@@ -500,3 +504,10 @@ def test_a_backward_pass_is_not_captured_beside_an_eager_graph_of_its_leaves(op)
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_the_policy_loop_runs_with_residual_blocks():
+    """The command's own network with norm_residual in it: acting in a graph, collecting, learning."""
+    r = subprocess.run([sys.executable, os.path.join(ROOT, "examples", "torch_policy_loop.py"), "--envs", "2048", "--steps", "40", "--blocks", "2"], capture_output=True, text=True, timeout=110)
+    assert r.returncode == 0, r.stderr[-2000:]
+    assert "act, learn, update" in r.stdout and "nan" not in r.stdout, r.stdout
