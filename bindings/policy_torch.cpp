@@ -69,9 +69,10 @@ void check(const char* name, const Tensor& t, at::IntArrayRef shape, const Tenso
 
 // What would vanish without a word: a call that torch.jit traces (it would record the empty output), a dual tensor's tangent.
 void not_traced(const char* what) { TORCH_CHECK(!torch::jit::tracer::isTracing(), what, " cannot be traced"); }
-void no_tangent(const char* what, const Tensor& t) {
-    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), what, " has no forward-mode derivative");
+void no_tangents(const char* what, std::initializer_list<const Tensor*> tensors) {
+    for (const Tensor* t : tensors) TORCH_CHECK_NOT_IMPLEMENTED(!t || !t->_fw_grad(0).defined(), what, " has no forward-mode derivative");
 }
+const Tensor* there(const OptTensor& t) { return t.has_value() && t->defined() ? &*t : nullptr; }
 
 bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
 OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }  // autograd takes absent tensors, not undefined ones
@@ -216,7 +217,7 @@ bool overlap(const Tensor& a, const Tensor& b) {
 Tensor linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, const std::string& activation, const OptTensor& residual, const OptTensor& out) {
     dtype_of(x, "x");
     not_traced("linear");
-    for (const Tensor& t : {x, weight, bias.value_or(Tensor()), residual.value_or(Tensor()), out.value_or(Tensor())}) no_tangent("linear", t);
+    no_tangents("linear", {&x, &weight, there(bias), there(residual), there(out)});
     const int act = activation_of(activation);
     TORCH_CHECK_VALUE(weight.dim() == 2 && x.dim() >= 1, "weight must be [out, in] and x [..., in], got ", weight.sizes(), " and ", x.sizes());
     const int64_t n = weight.size(0), k = weight.size(1);
@@ -325,7 +326,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
 std::tuple<Tensor, Tensor> norm_residual(const Tensor& x, const OptTensor& block, const OptTensor& gate, double scale, const OptTensor& post_weight, const OptTensor& pre_weight, double eps) {
     dtype_of(x, "x");
     not_traced("norm_residual");
-    for (const Tensor& t : {x, block.value_or(Tensor()), gate.value_or(Tensor()), post_weight.value_or(Tensor()), pre_weight.value_or(Tensor())}) no_tangent("norm_residual", t);
+    no_tangents("norm_residual", {&x, there(block), there(gate), there(post_weight), there(pre_weight)});
     TORCH_CHECK_VALUE(x.dim() >= 1, "x must be [..., width]");
     const int64_t width = x.size(-1);
     TORCH_CHECK_VALUE(width >= 1 && width <= 4096, "width must be 1 ... 4096, got ", width);
