@@ -121,8 +121,14 @@ class AdamW(torch.optim.Optimizer):
         their addresses, so that a captured step goes on from the loaded state."""
         mine = {p: self.state[p] for g in self.param_groups for p in g["params"]}
         steps = [g["step"] for g in self.param_groups]
-        super().load_state_dict(state_dict)
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        if len(saved) != len(mine) or not all("step" in g for g in state_dict["param_groups"]):
+            raise ValueError("the state is not one of these parameter groups")
+        for (p, state), i in zip(mine.items(), saved):
+            theirs = state_dict["state"].get(i, {})
+            if any(k not in theirs or theirs[k].shape != p.shape for k in state):
+                raise ValueError(f"the state of parameter {i} is not {', '.join(state)} of shape {tuple(p.shape)}")
+        super().load_state_dict(state_dict)
         for (p, state), i in zip(mine.items(), saved):
             for k, v in state.items():
                 v.copy_(state_dict["state"][i][k])

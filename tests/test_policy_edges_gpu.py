@@ -511,3 +511,43 @@ def test_the_policy_loop_runs_with_residual_blocks():
     r = subprocess.run([sys.executable, os.path.join(ROOT, "examples", "torch_policy_loop.py"), "--envs", "2048", "--steps", "40", "--blocks", "2"], capture_output=True, text=True, timeout=110)
     assert r.returncode == 0, r.stderr[-2000:]
     assert "act, learn, update" in r.stdout and "nan" not in r.stdout, r.stdout
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+def test_optimizer_refuses_a_state_that_is_not_its_own(t):
+    """A state of other shapes, of torch's AdamW or without its masters is refused before anything is written."""
+    def make():
+        ps = [torch.nn.Parameter(rand(6, 5, to=t, seed=1)), torch.nn.Parameter(rand(5, to=t, seed=2))]
+        for p in ps:
+            p.grad = torch.ones_like(p)
+        opt = policy.AdamW(ps, lr=1e-2)
+        opt.step()
+        return ps, opt
+
+    ps, opt = make()
+    good = opt.state_dict()
+    other = [torch.nn.Parameter(rand(6, 5, seed=1)), torch.nn.Parameter(rand(1, seed=2))]
+    theirs = torch.optim.AdamW(ps)
+    theirs.step()
+    bad = [theirs.state_dict()]
+    for key, value in (("exp_avg", torch.zeros(1, device="cuda")), ("exp_avg_sq", None)):
+        broken = {"param_groups": good["param_groups"], "state": {i: dict(s) for i, s in good["state"].items()}}
+        if value is None:
+            del broken["state"][1][key]
+        else:
+            broken["state"][1][key] = value
+        bad.append(broken)
+    bad.append(policy.AdamW(other).state_dict())
+    for state in bad:
+        with pytest.raises(ValueError, match="state"):
+            opt.load_state_dict(state)
+    twins, twin = make()
+    theirs_undone = [p.detach().clone() for p in twins]
+    with torch.no_grad():
+        for p, q in zip(ps, theirs_undone):
+            p.copy_(q)
+    opt.step()
+    twin.step()
+    assert all(torch.equal(p, q) for p, q in zip(ps, twins)) and opt.param_groups[0]["lr"] == 1e-2
+    opt.load_state_dict(good)
+    assert opt.param_groups[0]["step"].item() == 2
