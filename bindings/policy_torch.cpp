@@ -1,7 +1,7 @@
 // policy_torch.cpp — module drone_amd/policy_torch: the policy operators of include/drone_vec.h for torch tensors, with their
 // autograd nodes. Host code only (g++, libtorch): it checks tensors, fills the call structs and calls the C-ABI on torch's
 // current stream. Compiled rather than ctypes because what it saves is what small policies wait for: a forward call costs
-// about 4 us of host time instead of 12, forward + gradient about 30 instead of 130.
+// about 5 us of host time instead of 12, forward + gradient 40 to 60 (33 of them autograd's own two threads) instead of 130.
 // The library's entry points come from drone_amd.binding (bind()), so that DRONE_HIP_LIB and its load errors hold here too.
 #include <torch/extension.h>
 
@@ -195,8 +195,9 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
             if (wants & 1) { dx = at::empty({x.size(0), x.size(1)}, x.options()); c.dx = ptr(dx); c.dx_ld = x.size(1); }
             if (wants & 2) { dw = at::empty({w.size(0), w.size(1)}, x.options()); c.dweight = ptr(dw); }
             if (wants & 4) { db = at::empty({w.size(0)}, x.options()); c.dbias = ptr(db); }
-            // (dx alone needs none, but streams through one where the layer is wide)
-            if ((wants & 6) || w.numel() > 128 * 128) { work = workspace(lib.linear_workspace(&c), x); c.workspace = ptr(work); c.workspace_bytes = work.numel(); }
+            // (dx alone needs none, but streams through one where the layer is wide and whole 16-byte pieces)
+            const auto whole = [&](int64_t n) { return n * (int64_t)x.element_size() % 16 == 0; };
+            if ((wants & 6) || (w.numel() > 128 * 128 && whole(w.size(0)) && whole(w.size(1)))) { work = workspace(lib.linear_workspace(&c), x); c.workspace = ptr(work); c.workspace_bytes = work.numel(); }
             run(lib.linear_backward(&c, stream_of(x)));
         }
         return once({dx, dw, db, wants & 8 ? dys[0] : Tensor(), Tensor()}, "linear");

@@ -6,7 +6,8 @@
 // so that a captured step replays with an advancing t), then the update; one launch of one workgroup where all the tensors
 // together are a few chunks (the six tensors of a 20-64-64-4 policy: 7.8 us, 9.6 in two). Everything in 32 bits; a 16-bit
 // weight is its 32-bit master rounded once, and the master is what the next step starts from unless the weight is no longer
-// that. Bound by memory: 21e6 16-bit weights with masters, 672 MB, 135 us (5.0 TB/s; a copy reaches 5.1; the norm has to have read every gradient before the first update, and reads them from the cache's leavings again).
+// that. Bound by memory: 21e6 16-bit weights with masters, 672 MB, 23 + 114 us (4.9 TB/s; a copy reaches 5.1; the norm has to
+// have read every gradient before the first update, and reads them from the cache's leavings again).
 #include <hip/hip_runtime.h>
 
 #include "drone_policy.hpp"
@@ -75,7 +76,8 @@ __global__ __launch_bounds__(kThreads) void adamw_norm_kernel(AdamwArgs a) {
         if (a.norm && !a.chunks) *a.norm = 0.f;  // no gradients at all
     }
     if (!a.parts) return;
-    double sum = 0;  // a thread of the largest calls adds up 131 072 squares: in 32 bits equal ones were rounded alike, 9e-6 off at 2 048
+    // 64 bits: a thread of the largest calls adds up 131 072 squares (in 32, 2 048 equal ones were rounded alike, 9e-6 off)
+    double sum = 0;
     for (int chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
         const AdamwTensor& t = a.t[tensor_of(a, chunk)];
         float g[8];
@@ -112,8 +114,7 @@ struct Eight {
         load8((const T*)t.p, i, t.n, t.vec, p);
         if (sizeof(T) == 4) return;
         // A 16-bit weight that is not its rounded master has been written since the last step (a loaded state, a target's
-        // copy): the step starts from it. The two bytes more cost 21e6
-        // weights 8 us (135 against 127).
+        // copy): the step starts from it. The two bytes more cost 21e6 weights 8 us (135 against 127).
         float master[8];
         load8(t.master, i, t.n, t.vec, master);
 #pragma unroll

@@ -2,7 +2,8 @@
 
 The env's observations, rewards and flags stay in HBM (``DroneVec`` with a device); what a learner runs between two env
 steps are many-row, narrow layers and an update of a dozen small tensors, where launches and passes over memory are the
-cost. Three operators over the C-ABI of ``include/drone_vec.h``, each one or two launches on torch's current stream:
+cost. Three operators over the C-ABI of ``include/drone_vec.h``, on torch's current stream; a forward call is one launch, the
+gradient of norms one or two, that of a layer two (narrow) to six (odd widths), the optimizer step one or two:
 
 * ``linear``: ``y = act(x W^T + b) + residual`` (``drone_linear_forward`` / ``_backward``)
 * ``norm_residual``: the norms after and before a block, its gate and residual scale (``drone_norm_forward`` / ``_backward``)
@@ -43,7 +44,8 @@ def linear(x, weight, bias=None, activation="none", residual=None, out=None):
 
     x ``[..., in]``, weight ``[out, in]``, bias ``[out]``, residual ``[..., out]``, one type (float32, bfloat16, float16)
     and one GPU; activation: none, relu, tanh, silu, gelu (the erf form). Sums are 32-bit, the result is rounded once; calls of
-    one shape give the same bits, another number of rows may sum in another order.
+    one shape give the same bits, another number of rows may sum in another order. The gradient rounds dy act'(z) to the type
+    once more for its products: 16-bit dx and dweight are 1.4 times as far off as their own rounding.
     ``out``: a tensor to write instead of a new one (the env's action buffer), ``[..., out]`` with contiguous rows; only
     where nothing is differentiated; it may be the residual. Rows may be a strided view; anything else is copied first."""
     return _native().linear(x, weight, bias, activation, residual, out)
@@ -57,20 +59,20 @@ def norm_residual(x, block=None, *, gate=None, scale=1.0, post_weight=None, pre_
 
     ``r`` is the residual stream behind the block, ``h`` what the next block reads. x, block ``[..., width]``; gate
     ``[width]`` or ``[..., width]`` or None (1); weights ``[width]`` or None (1); width 1 ... 4096. Without a block
-    ``r = x``. Differentiable (once, backward) in all five tensors; scale and eps are
-    numbers."""
+    ``r = x``. Differentiable (once, backward) in all five tensors; scale and eps are numbers."""
     return _native().norm_residual(x, block, gate, scale, post_weight, pre_weight, eps)
 
 
 @torch.no_grad()
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, max_grad_norm=None, masters=None):
-    """One AdamW step over all tensors, in place, two launches (one where all tensors
-    together are a few thousand values); returns the gradients' global norm before clipping
-    (``[1]`` float32 on the device). ``max_grad_norm``: scale the gradients by ``min(1, max_grad_norm / (norm + 1e-6))``.
+    """One AdamW step over all tensors, in place, two launches (one where all tensors together are a few thousand values);
+    returns the gradients' global norm before clipping (``[1]`` float32 on the device). ``max_grad_norm`` (positive): scale
+    the gradients by ``min(1, max_grad_norm / (norm + 1e-6))``.
 
     params and grads of one type; exp_avgs, exp_avg_sqs float32; 16-bit params need float32 ``masters`` (the params are
-    their rounded copies; a value that is not has been written since, and the step starts from it). ``step``: int32 tensor ``[1]`` on the device, the steps done so far; the call adds 1, so a step
-    captured into a graph replays with an advancing count. All tensors contiguous, on one GPU, none twice or over another."""
+    their rounded copies; a value that is not has been written since, and the step starts from it). ``step``: int32 tensor
+    ``[1]`` on the device, the steps done so far; the call adds 1, so a step captured into a graph replays with an advancing
+    count. All tensors contiguous, on one GPU, none twice or over another."""
     return _native().adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas, eps, weight_decay, max_grad_norm, masters)
 
 
@@ -88,7 +90,8 @@ class AdamW(torch.optim.Optimizer):
     parameters) masters in float32. Weights may be written between steps (a loaded state, a target network's copy): the next
     step starts from what is there. ``max_grad_norm`` clips by the norm over a whole group; ``grad_norm`` holds the last
     step's norms, one ``[1]`` tensor per group (None where no parameter had a gradient). Parameters without a gradient are
-    left alone; the step count is the group's. ``lr`` and the rest are read at every call (a captured step keeps those of its capture)."""
+    left alone; the step count is the group's. ``lr`` and the rest are read at every call (a captured step keeps those of
+    its capture)."""
 
     def __init__(self, params, lr=3e-4, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, max_grad_norm=None):
         if lr < 0 or weight_decay < 0 or not eps > 0 or not all(0 <= b < 1 for b in betas):

@@ -428,10 +428,11 @@ uint64_t drone_norm_workspace(const DroneNorm* call);
  *   m = beta1 m + (1 - beta1) g';  v = beta2 v + (1 - beta2) g'^2
  *   p = p (1 - lr weight_decay) - lr (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps)
  * p and g of `dtype`, m and v f32, master f32 (required for the 16-bit types, whose p is the rounded master: a p that is
- * not has been written since the last step, and the step starts from it; NULL for DRONE_F32), each dense with `elements` values. `step` (device, one int32) counts the steps done: the call adds 1 and t is
- * the result, so a captured call replays with an advancing t (lr and the rest stay those of the capture). `grad_norm`
- * (device, one f32) or NULL receives the norm before clipping. `tensors` is host memory, read during the call. No tensor
- * may appear twice or overlap another; elements 0 ... 2^34; eps > 0 and a normal f32. drone_adamw_workspace bytes at `workspace`. */
+ * not has been written since the last step, and the step starts from it; NULL for DRONE_F32), each dense with `elements`
+ * values. `step` (device, one int32) counts the steps done: the call adds 1 and t is the result, so a captured call replays
+ * with an advancing t (lr and the rest stay those of the capture). `grad_norm` (device, one f32) or NULL receives the norm
+ * before clipping. `tensors` is host memory, read during the call. No tensor may appear twice or overlap another; elements
+ * 0 ... 2^34; eps > 0 and a normal f32. drone_adamw_workspace bytes at `workspace`. */
 typedef struct DroneAdamWTensor {
     void* param;
     const void* grad;
