@@ -119,7 +119,11 @@ int64_t wanted(const AutogradContext* ctx, int64_t there) {
 // holds. It would run on that stream, where a capture cannot follow, and torch ends the process over it.
 void capturable(const Tensor& x, const char* what) {
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(c10::hip::getCurrentHIPStream(x.get_device()), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    if (hipStreamIsCapturing(c10::hip::getCurrentHIPStream(x.get_device()), &status) != hipSuccess) {
+        (void)hipGetLastError();  // (the null stream beside someone else's capture: not this pass's error, and not the next call's)
+        return;
+    }
+    if (status == hipStreamCaptureStatusNone) return;
     const auto node = torch::autograd::get_current_node();
     for (size_t i = 0; i < node->num_outputs(); i++) {
         const auto& leaf = node->next_edge(i).function;
